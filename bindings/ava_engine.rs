@@ -48,6 +48,23 @@ pub struct AvaConfig {
     pub slope: f32,
 }
 
+/// Keys and values in pages: element (page, head, place, channel) lies at page * page_stride + head * head_stride +
+/// place * place_stride + channel, counted in elements; `k` and `v` are device pointers.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct AvaPagedStore {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub dtype: i32,
+    pub n_pages: i32,
+    pub kv_heads: i32,
+    pub page_size: i32,
+    pub head_size: i32,
+    pub page_stride: i64,
+    pub head_stride: i64,
+    pub place_stride: i64,
+}
+
 #[repr(C)]
 pub struct AvaEngine { _p: [u8; 0] }
 #[repr(C)]
@@ -156,6 +173,12 @@ extern "C" {
     pub fn ava_op_tc_bgemm(device: c_int, batch: i32, m: i32, n: i32, k: i32, a: *const f32, b: *const f32, colscale: *const f32, c: *mut f32, c_limb_sum: *mut f32) -> c_int;
     pub fn ava_op_mem_chunk(device: c_int, t: i32, hb: i32, hs: i32, qn: *const f32, e: *const f32, w: *const f32, ah: *const f32, v: *const f32, la: *const f32, f: *mut f32, y: *mut f32, out_of_range: *mut i32) -> c_int;
     pub fn ava_debug_mem_heads_wait_runs_out(device: c_int, m: i32, hs: i32, chunk: i32, poll_limit: u32, state_changed: *mut i32) -> c_int;
+    pub fn ava_serving_last_error() -> *const c_char;
+    pub fn ava_paged_plan(device: c_int, stream: *mut c_void, cached: *const i32, fresh: *const i32, rows: i32, page_size: i32, n_pages: i32, table: *mut i32, max_pages: i32, owned: *const i32, owned_out: *mut i32, free_list: *mut i32, free_count: *const i32, free_count_out: *mut i32, trim: i32, q_start: *mut i32, slot: *mut i64, pos: *mut i32, row: *mut i32, max_tokens: i32, status: *mut u32) -> c_int;
+    pub fn ava_paged_append(device: c_int, stream: *mut c_void, store: *const AvaPagedStore, k: *const c_void, v: *const c_void, dtype: i32, token_stride: i64, head_stride: i64, slot: *const i64, tokens: i32, status: *mut u32) -> c_int;
+    pub fn ava_paged_attend_workspace(device: c_int, head_size: i32) -> i64;
+    pub fn ava_paged_attend(device: c_int, stream: *mut c_void, store: *const AvaPagedStore, q: *const c_void, dtype: i32, q_token_stride: i64, q_head_stride: i64, heads: i32, table: *const i32, max_pages: i32, cached: *const i32, first: *const i32, q_start: *const i32, rows: i32, max_tokens: i32, max_fresh: i32, scale: f32, window: i32, out: *mut c_void, out_token_stride: i64, out_head_stride: i64, lse: *mut f32, workspace: *mut c_void, workspace_bytes: i64, status: *mut u32) -> c_int;
+    pub fn ava_verify_drafts(device: c_int, stream: *mut c_void, p: *const f32, p_stride: i64, q: *const f32, q_stride: i64, tok: *const u32, q_start: *const i32, rows: i32, max_tokens: i32, vocab: i32, uniform: *const f64, max_out: i32, out: *mut u32, n_out: *mut i32, status: *mut u32) -> c_int;
     pub fn ava_host_expf(x: f32) -> f32;
     pub fn ava_host_logf(x: f32) -> f32;
     pub fn ava_host_rsqrtf(x: f32) -> f32;

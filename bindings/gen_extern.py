@@ -19,7 +19,8 @@ END = "    // ---- end: generated"
 
 BASE = {"int": "c_int", "int32_t": "i32", "int64_t": "i64", "uint32_t": "u32", "uint64_t": "u64", "uint8_t": "u8", "int8_t": "i8",
         "unsigned char": "u8", "float": "f32", "double": "f64", "char": "c_char", "void": "c_void", "size_t": "usize",
-        "ava_engine": "AvaEngine", "ava_state": "AvaState", "ava_ckpt": "AvaCkpt", "ava_trace": "AvaTrace", "ava_config": "AvaConfig"}
+        "ava_engine": "AvaEngine", "ava_state": "AvaState", "ava_ckpt": "AvaCkpt", "ava_trace": "AvaTrace", "ava_config": "AvaConfig",
+        "ava_paged_store": "AvaPagedStore"}
 CALLBACKS = {"ava_pick_fn": "Option<extern \"C\" fn(*mut c_void, i32, *const f32, i32) -> u32>",
              "ava_stop_fn": "Option<extern \"C\" fn(*mut c_void, i32, *const u32, i32) -> c_int>"}
 RUST_KEYWORDS = {"type", "in", "ref", "box", "move", "fn", "impl", "loop", "match", "mod", "use", "where", "self"}

@@ -476,6 +476,114 @@ int ava_op_mem_chunk(int device, int32_t t, int32_t hb, int32_t hs, const float*
  * *state_changed = 1 if any bit of the state in device memory changed (a block that gave up must store nothing). */
 int ava_debug_mem_heads_wait_runs_out(int device, int32_t m, int32_t hs, int32_t chunk, uint32_t poll_limit, int32_t* state_changed);
 
+/* ---- serving from pages ------------------------------------------------------------------------------------------
+ * No counterpart in the reference (one growing store per row, src/state.rs:46-49, read once per token,
+ * src/model/fstep.rs:303-356; one token drawn per step, src/diary.rs:686-718).  Four operators that one scheduling step
+ * of a server runs one after another, on requests of different lengths whose keys and values lie in fixed-size pages:
+ *   ava_paged_plan     the step's block tables and slot maps, built on the GPU from the requests' lengths
+ *   ava_paged_append   the new tokens' keys and values join their pages
+ *   ava_paged_attend   the new tokens read their requests' pages (a whole prompt chunk, a drafted run or a single token)
+ *   ava_verify_drafts  drafted tokens held against the target's probabilities
+ *
+ * Every pointer is DEVICE memory of `device` unless it says host; `stream` is a cudaStream_t of that device (NULL: its
+ * default stream).  The calls queue their kernels and return: no allocation, no host copy, no wait; all of them may be
+ * captured into a CUDA graph (the lengths are read on the GPU, so a replay follows them).  The calling thread's current
+ * device is left as it was.  Different threads may call at once (each call's arrays are its caller's).
+ * Argument errors are found before anything is queued (AVA_ERR_ARG, or AVA_NOT_APPLICABLE for a shape or type that is
+ * not covered; text from ava_serving_last_error, per thread).  What only the GPU can see in the arrays is reported in a
+ * status word: each operator checks every index it takes from an array, never touches memory outside the arrays it was
+ * given, and ORs what it found into status[0] (ava_paged_plan sets it).  status may be NULL. */
+#define AVA_F32 0
+#define AVA_BF16 1
+#define AVA_PAGED_NO_PAGES 1u      /* the free list holds fewer pages than the step needs */
+#define AVA_PAGED_NO_TABLE 2u      /* a request needs more pages than its row of the table has places */
+#define AVA_PAGED_BAD_LENGTH 4u    /* a negative length, counts that do not fit the arrays, or q_start not ascending */
+#define AVA_PAGED_NO_TOKENS 8u     /* more new tokens than max_tokens */
+#define AVA_PAGED_BAD_PAGE 16u     /* a page or slot outside the store */
+#define AVA_PAGED_BAD_TOKEN 32u    /* a drafted token outside the vocabulary */
+#define AVA_PAGED_NO_MASS 64u      /* probabilities that sum to nothing, or not to a finite number */
+#define AVA_NO_TOKEN 0xffffffffu
+/* Text of the last argument or launch error of these calls on this thread (never NULL). */
+const char* ava_serving_last_error(void);
+
+/* Keys and values in pages (this struct itself is host memory): element (page, head, place, channel) of either lies at
+ * page * page_stride + head * head_stride + place * place_stride + channel, counted in elements. */
+typedef struct ava_paged_store {
+    void* k;
+    void* v;
+    int32_t dtype;          /* AVA_F32 or AVA_BF16, both pools */
+    int32_t n_pages;
+    int32_t kv_heads;
+    int32_t page_size;      /* tokens per page, any number >= 1 */
+    int32_t head_size;
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t place_stride;
+} ava_paged_store;
+
+/* One step's lists.  Request r holds cached[r] tokens and adds fresh[r] now (0: none); it owns the first owned[r] entries
+ * of its row of table [rows][max_pages].  free_list [n_pages] is a stack of the free pages, free_count [1] its height.
+ *   need(r) = ceil((cached[r] + fresh[r]) / page_size)
+ *   trim != 0: the pages of a request beyond need(r) go on the stack, in the order of request and place (a request with
+ *     no tokens left gives all of them back); trim == 0: they stay its own (room for the next drafted run)
+ *   then every request takes what it lacks off the stack's top, in the order of request and place: new table entries
+ * owned_out [rows] and free_count_out [1] get the new counts (either may be its own input: in place), q_start [rows + 1]
+ * the first new token of every request in the packed order of this step, and per new token slot (page * page_size +
+ * place), pos (its position in its request) and row (its request); pos and row may be NULL.  Places behind the last
+ * token, up to max_tokens, get -1 in all three, so a batch of fixed size runs through the other operators as it is.
+ * Table entries that are neither taken nor owned are left as they are.  All or nothing: when the status word is not 0
+ * (NO_PAGES, NO_TABLE, BAD_LENGTH, NO_TOKENS) no page changes hands, the counts are copied, q_start is all 0 and slot,
+ * pos and row are all -1.  A page number outside 0 .. n_pages - 1 in the list or the table: BAD_PAGE, and -1 as the slot
+ * of its tokens. */
+int ava_paged_plan(int device, void* stream, const int32_t* cached, const int32_t* fresh, int32_t rows, int32_t page_size, int32_t n_pages,
+                   int32_t* table, int32_t max_pages, const int32_t* owned, int32_t* owned_out, int32_t* free_list, const int32_t* free_count,
+                   int32_t* free_count_out, int32_t trim, int32_t* q_start, int64_t* slot, int32_t* pos, int32_t* row, int32_t max_tokens,
+                   uint32_t* status);
+
+/* The keys and values of `tokens` new tokens into the store: k and v (dtype; element (token, head, channel) of either at
+ * token * token_stride + head * head_stride + channel) to the places slot[token] names; a negative slot is passed over.  f32 rows may go into
+ * an f32 or a bf16 store (rounded once, to nearest even), bf16 rows into a bf16 store; else AVA_NOT_APPLICABLE.  Slots are
+ * to be distinct: of two tokens with the same slot either's bytes may stay. */
+int ava_paged_append(int device, void* stream, const ava_paged_store* store, const void* k, const void* v, int32_t dtype, int64_t token_stride,
+                     int64_t head_stride, const int64_t* slot, int32_t tokens, uint32_t* status);
+
+/* The read of the new tokens, whose keys and values are in the store already: token i of request r (packed at
+ * q_start[r] + i, at position p = cached[r] + i) sees the keys first[r] .. p of its request (first NULL: 0), of them the
+ * last `window` when window > 0, and gets, per head h with key head h / (heads / kv_heads),
+ *   out = sum_j softmax_j(scale q . k_j) v_j,   lse = ln sum_j exp(scale q . k_j)   (lse [tokens][heads] f32, may be NULL)
+ * A token that sees no key gets zeros and -infinity.  out and lse of packed places from q_start[rows] on are left as they
+ * are.  q and out (dtype) have strides of their own, in elements, channels adjacent.  (q, store) types covered: f32 with
+ * f32, f32 with bf16, bf16 with bf16; head sizes 32, 64 and 128; else AVA_NOT_APPLICABLE.  Sums, maxima and the mix are
+ * f32; where products run on bf16 tensor cores f32 operands are carried as two bf16 limbs (a relative 2^-17 each), and
+ * with bf16 q the softmax weights are rounded to bf16 for their product with the values.
+ * max_fresh: the largest number of new tokens of a request, as the host knows it; it only chooses the kernel, and a
+ * longer request is read in full all the same.  max_tokens: rows of q and out.
+ * workspace: ava_paged_attend_workspace(device, head_size) bytes, 16-byte aligned, contents arbitrary and not kept from
+ * one call to the next; calls (or captured graphs) that may overlap on the GPU need one each. */
+int64_t ava_paged_attend_workspace(int device, int32_t head_size);
+int ava_paged_attend(int device, void* stream, const ava_paged_store* store, const void* q, int32_t dtype, int64_t q_token_stride,
+                     int64_t q_head_stride, int32_t heads, const int32_t* table, int32_t max_pages, const int32_t* cached, const int32_t* first,
+                     const int32_t* q_start, int32_t rows, int32_t max_tokens, int32_t max_fresh, float scale, int32_t window, void* out,
+                     int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace, int64_t workspace_bytes, uint32_t* status);
+
+/* Request r fed q_start[r + 1] - q_start[r] = n + 1 tokens: the last one it was given and n drafted ones, tok[q_start[r] + 1 + i]
+ * the i-th; row q_start[r] + i of p (f32 [max_tokens], row stride p_stride) holds the target's probabilities behind that
+ * token, the same row of q those the i-th draft was drawn from (q NULL: the draft is certain, q(d) = 1).
+ *   accepted, while all before it were:  uniform[q_start[r] + i] * q(d) < p(d)
+ *   the token behind the accepted ones is drawn from max(p - q, 0) of the refused draft's row (q NULL: p without the draft;
+ *   all accepted: p of the last row): the lowest token whose running sum, in token order, exceeds
+ *   uniform[q_start[r] + n] * the whole sum
+ * so that the tokens are distributed as the target's own.  Products and sums in f64; a probability that is negative or NaN
+ * counts as 0; a difference without mass falls back to p, p without mass gives AVA_NO_TOKEN and NO_MASS.  uniform NULL:
+ * greedy, p may be logits; a draft is accepted while it is its row's largest value (lowest token among equals, NaN never),
+ * and the token behind is the largest of its row.
+ * out [rows][max_out] gets the accepted drafts and the token behind them, AVA_NO_TOKEN in the places that are left; n_out
+ * [rows] their number (0 for a request that fed nothing), which is also what cached[r] grows by.  A request with more
+ * than max_out - 1 drafts: BAD_LENGTH, n_out 0. */
+int ava_verify_drafts(int device, void* stream, const float* p, int64_t p_stride, const float* q, int64_t q_stride, const uint32_t* tok,
+                      const int32_t* q_start, int32_t rows, int32_t max_tokens, int32_t vocab, const double* uniform, int32_t max_out, uint32_t* out,
+                      int32_t* n_out, uint32_t* status);
+
 /* The engine's exp / ln / x^-1/2, evaluated on the host with the operation sequence the kernels use (same bits). */
 float ava_host_expf(float x);
 float ava_host_logf(float x);
