@@ -55,6 +55,11 @@ int launched(cudaError_t rc, const char* call) {
     return fail(AVA_ERR_CUDA, call, cudaGetErrorString(rc));
 }
 
+int sm_count(int device) {
+    int n = 0;
+    return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess ? n : 0;
+}
+
 // What append and attend need of a store; nullptr: fine.
 const char* store_fault(const ava_paged_store* s) {
     if (!s || !s->k || !s->v) return "a store without its pools";
@@ -120,7 +125,9 @@ int64_t ava_paged_attend_workspace(int device, int32_t head_size) {
     if (head_size != 32 && head_size != 64 && head_size != 128) return fail(AVA_NOT_APPLICABLE, call, "head sizes 32, 64 and 128"), -1;
     OnDevice dev(device);
     if (!dev.ok) return fail(AVA_ERR_CUDA, call, NO_DEVICE), -1;
-    return 16;
+    const int sms = sm_count(device);
+    if (sms <= 0) return fail(AVA_ERR_CUDA, call, NO_DEVICE), -1;
+    return paged_read_workspace(head_size, sms);
 }
 
 int ava_paged_attend(int device, void* stream, const ava_paged_store* store, const void* q, int32_t dtype, int64_t q_token_stride,
@@ -142,20 +149,24 @@ int ava_paged_attend(int device, void* stream, const ava_paged_store* store, con
     for (const void* w : words)
         if (!aligned(w, 4)) return fail(AVA_ERR_ARG, call, "lists, lse and status must be 4-byte aligned");
     if (store->head_size != 32 && store->head_size != 64 && store->head_size != 128) return fail(AVA_NOT_APPLICABLE, call, "head sizes 32, 64 and 128");
+    // the store is read in pieces of 16 bytes
+    const int64_t piece = store->dtype == AVA_BF16 ? 8 : 4;
+    if (!aligned(store->k, 16) || !aligned(store->v, 16) || store->page_stride % piece || store->head_stride % piece || store->place_stride % piece)
+        return fail(AVA_ERR_ARG, call, "the store's pools and strides must be multiples of 16 bytes");
     if (dtype == AVA_BF16 && store->dtype == AVA_F32) return fail(AVA_NOT_APPLICABLE, call, "bf16 queries over an f32 store");
     OnDevice dev(device);
     if (!dev.ok) return fail(AVA_ERR_CUDA, call, NO_DEVICE);
-    const int64_t need = ava_paged_attend_workspace(device, store->head_size);
-    if (need < 0) return AVA_ERR_CUDA;
-    if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) return fail(AVA_ERR_ARG, call, "workspace: too small, missing or not 16-byte aligned");
+    const int sms = sm_count(device);
+    if (sms <= 0) return fail(AVA_ERR_CUDA, call, NO_DEVICE);
+    if (!workspace || workspace_bytes < paged_read_workspace(store->head_size, sms) || !aligned(workspace, 16)) return fail(AVA_ERR_ARG, call, "workspace: too small, missing or not 16-byte aligned");
     if (max_tokens == 0) return AVA_OK;
     ReadArgs a{};
     a.s = *store; a.q = q; a.out = out; a.lse = lse;
     a.q_token_stride = q_token_stride; a.q_head_stride = q_head_stride; a.out_token_stride = out_token_stride; a.out_head_stride = out_head_stride;
     a.table = table; a.cached = cached; a.first = first; a.q_start = q_start; a.status = status; a.scale = scale;
-    a.heads = heads; a.group = heads / store->kv_heads; a.max_pages = max_pages; a.rows = rows; a.max_tokens = max_tokens; a.window = window;
-    a.bf16_q = dtype == AVA_BF16;
-    return launched(launch_paged_read(static_cast<cudaStream_t>(stream), a), call);
+    a.heads = heads; a.group = heads / store->kv_heads; a.max_pages = max_pages; a.rows = rows; a.max_tokens = max_tokens; a.max_fresh = max_fresh;
+    a.window = window; a.bf16_q = dtype == AVA_BF16;
+    return launched(launch_paged_read(static_cast<cudaStream_t>(stream), a, workspace, sms), call);
 }
 
 int ava_verify_drafts(int device, void* stream, const float* p, int64_t p_stride, const float* q, int64_t q_stride, const uint32_t* tok,

@@ -65,9 +65,11 @@ struct ReadArgs {
     const int32_t *table, *cached, *first, *q_start;
     uint32_t* status;
     float scale;
-    int heads, group, max_pages, rows, max_tokens, window, bf16_q;
+    int heads, group, max_pages, rows, max_tokens, max_fresh, window, bf16_q;
 };
-cudaError_t launch_paged_read(cudaStream_t st, const ReadArgs& a);
+// room: paged_read_workspace bytes
+cudaError_t launch_paged_read(cudaStream_t st, const ReadArgs& a, void* room, int sms);
+int64_t paged_read_workspace(int head_size, int sms);
 
 // ---- drafted tokens (k_verify.cu)
 struct VerifyArgs {

@@ -554,8 +554,9 @@ int ava_paged_append(int device, void* stream, const ava_paged_store* store, con
  * A token that sees no key gets zeros and -infinity.  out and lse of packed places from q_start[rows] on are left as they
  * are.  q and out (dtype) have strides of their own, in elements, channels adjacent.  (q, store) types covered: f32 with
  * f32, f32 with bf16, bf16 with bf16; head sizes 32, 64 and 128; else AVA_NOT_APPLICABLE.  Sums, maxima and the mix are
- * f32; where products run on bf16 tensor cores f32 operands are carried as two bf16 limbs (a relative 2^-17 each), and
- * with bf16 q the softmax weights are rounded to bf16 for their product with the values.
+ * f32; the products run on bf16 tensor cores with f32 operands carried as three bf16 limbs (2^-24 of each), and with
+ * bf16 q the softmax weights are rounded to bf16 for their product with the values.  The pools and their strides must be
+ * multiples of 16 bytes.  What a request on a page outside the store reads (BAD_PAGE) means nothing.
  * max_fresh: the largest number of new tokens of a request, as the host knows it; it only chooses the kernel, and a
  * longer request is read in full all the same.  max_tokens: rows of q and out.
  * workspace: ava_paged_attend_workspace(device, head_size) bytes, 16-byte aligned, contents arbitrary and not kept from

@@ -1,13 +1,14 @@
 """The serving operators against plain 64-bit implementations, at the sizes and masks where they can go wrong.
 
-Tolerances.  attend: a score is a sum of head_size products in f32 of operands carried to a relative 2^-17 at worst (two
-bf16 limbs; exact where the operand is bf16), so it is off by at most
-    ds = |scale| sum|q||k| (2^-17 [q is f32] + 2^-17 [the store is f32] + 2^-17 [both: the product of the low limbs is left out] + (head_size + 2) 2^-24)
+Tolerances.  attend: operands are carried as bf16 limbs to 2^-24 (products of limbs below 2^-26 left out: 2^-24 of the
+product for three of them) and products are summed in f32 whose last bit may be cut instead of rounded, so a score is off by
+at most
+    ds = |scale| sum|q||k| (head_size + 16) 2^-23
 and by the rounding of its exponent's argument and of the exponential itself, (|s - max| + 4) 2^-23.  A weight is then off
-by a relative dw = ds + ds(max) + (|s - max| + 4) 2^-23, and an output by sum w|v| (2 dw + dp + (keys + 8) 2^-24), with
-dp = 2^-17 for a weight carried as two limbs (+ 2^-16 for an f32 store: its values as limbs, the low product left out) or
-2^-8 for one rounded to bf16 (half a step; the sum of the weights is taken before that), and half a step of the output's own
-type.  The logarithm of the sum moves with its scores: max ds + (max|s - max| + keys + 8) 2^-23 + |lse| 2^-23.
+by a relative dw = ds + ds(max) + (|s - max| + 4) 2^-23, and an output by sum w|v| (2 dw + dp + (keys + 16) 2^-23), with
+dp = 2^-23 for limbed weights or 2^-8 for one rounded to bf16 (half a step; the sum of the weights is taken before that),
+and half a step of the output's own type.  The logarithm of the sum moves with its scores:
+max ds + (max|s - max| + keys + 8) 2^-23 + |lse| 2^-23.
 Everything else is equal to the bit: lists, slots, tokens, and a bf16 rounding."""
 import numpy as np
 import pytest
@@ -302,7 +303,7 @@ def call_attend(T, S, x, scale, window=0, max_fresh=None, status=None, room=None
 
 
 def check_attend(T, x, out, lse, scale, window=0, only=None):
-    f32q, f32s = x["dt"].startswith("f32"), x["dt"].endswith("f32")
+    f32q = x["dt"].startswith("f32")
     hs, at = x["q"].shape[2], 0
     for r, (c, f) in enumerate(x["lengths"]):
         if f and (only is None or r in only):
@@ -321,12 +322,11 @@ def check_attend(T, x, out, lse, scale, window=0, only=None):
             w = e / total.clamp(min=1e-300)
             want_lse = T.where(total > 0, top + total.log(), -float("inf"))[..., 0]
             want = w @ v
-            lost = 2.0 ** -17 * (f32q + f32s + (f32q and f32s)) + (hs + 2) * 2.0 ** -24
-            ds = abs(scale) * (q.abs() @ k.abs().transpose(1, 2)) * lost
+            ds = abs(scale) * (q.abs() @ k.abs().transpose(1, 2)) * (hs + 16) * 2.0 ** -23
             ds_top = ds.masked_fill(~seen, 0.0).amax(-1, keepdim=True)
             dw = ds + ds_top + ((s - top).abs().masked_fill(~seen, 0.0) + 4) * 2.0 ** -23
-            dp = 2.0 ** -17 + (2.0 ** -16 if f32s else 0.0) if f32q else 2.0 ** -8
-            tol = (w * (2 * dw + dp + (c + f + 8) * 2.0 ** -24)) @ v.abs() + 1e-30
+            dp = 2.0 ** -23 if f32q else 2.0 ** -8
+            tol = (w * (2 * dw + dp + (c + f + 16) * 2.0 ** -23)) @ v.abs() + 1e-30
             got = out[at:at + f].double().transpose(0, 1)
             if not f32q:
                 tol = tol + (want.abs() + tol) * 2.0 ** -8
