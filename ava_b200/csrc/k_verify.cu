@@ -35,44 +35,59 @@ __device__ __forceinline__ double weight(float p, float q) {
     return fmax(x - y, 0.0);
 }
 
-// weights of tokens j .. j + 3 (those at or beyond hi count nothing)
-__device__ __forceinline__ void weights4(const Row& w, int j, int hi, bool wide, double (&x)[4]) {
-    float p[4], q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+// p and q of tokens j .. j + 3 (those at or beyond hi read as 0)
+__device__ __forceinline__ void load4(const Row& w, int j, int hi, bool wide, float (&p)[4], float (&q)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = q[i] = 0.0f;
     if (wide && j + 4 <= hi) {
-        const float4 u = *reinterpret_cast<const float4*>(w.p + j);
+        const float4 u = __ldg(reinterpret_cast<const float4*>(w.p + j));
         p[0] = u.x; p[1] = u.y; p[2] = u.z; p[3] = u.w;
         if (w.q) {
-            const float4 v = *reinterpret_cast<const float4*>(w.q + j);
+            const float4 v = __ldg(reinterpret_cast<const float4*>(w.q + j));
             q[0] = v.x; q[1] = v.y; q[2] = v.z; q[3] = v.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            p[i] = j + i < hi ? w.p[j + i] : 0.0f;
-            if (w.q) q[i] = j + i < hi ? w.q[j + i] : 0.0f;
-        }
+        for (int i = 0; i < 4; ++i)
+            if (j + i < hi) {
+                p[i] = __ldg(w.p + j + i);
+                if (w.q) q[i] = __ldg(w.q + j + i);
+            }
     }
+}
+__device__ __forceinline__ void weights4(const Row& w, int j, const float (&p)[4], const float (&q)[4], double (&x)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = j + i == w.without ? 0.0 : weight(p[i], q[i]);
 }
 
-// The block's part [lo, hi) in tiles of 128 * m tokens, one warp each: their sums.
+// The block's part [lo, hi) in tiles of 128 * m tokens: their sums.  A warp walks its V_TILES / V_WARPS tiles together, so
+// that their loads are in flight at once (one tile after the other waited for memory tile by tile: 63 us for 256 requests
+// of 32768 tokens).
 __device__ __forceinline__ void tile_sums(const Row& w, int lo, int hi, int m, bool wide, double* sums) {
+    constexpr int MINE = V_TILES / V_WARPS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int t = warp; t < V_TILES; t += V_WARPS) {
-        double s = 0.0;
-        const int at = lo + t * 128 * m;
-        for (int b = 0; b < m; ++b) {
-            const int j = at + b * 128 + lane * 4;
-            if (j >= hi) break;
-            double x[4];
-            weights4(w, j, hi, wide, x);
-            s += (x[0] + x[1]) + (x[2] + x[3]);
-        }
+    double s[MINE];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) sums[t] = s;
+    for (int k = 0; k < MINE; ++k) s[k] = 0.0;
+#pragma unroll 2
+    for (int b = 0; b < m; ++b) {
+        float p[MINE][4], q[MINE][4];
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) load4(w, lo + ((warp * MINE + k) * m + b) * 128 + lane * 4, hi, wide, p[k], q[k]);
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            double x[4];
+            weights4(w, lo + ((warp * MINE + k) * m + b) * 128 + lane * 4, p[k], q[k], x);
+            s[k] += (x[0] + x[1]) + (x[2] + x[3]);
+        }
     }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+    if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) sums[warp * MINE + k] = s[k];
 }
 
 __global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
@@ -248,8 +263,10 @@ __global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
         int pick = -1, last = -1;
         for (int b = 0; b < m && pick < 0; ++b) {
             const int j = lo + tile * 128 * m + b * 128 + lane * 4;
-            double x[4] = {0.0, 0.0, 0.0, 0.0};
-            if (j < hi) weights4(w, j, hi, wide, x);
+            float p[4], q[4];
+            double x[4];
+            load4(w, j, hi, wide, p, q);
+            weights4(w, j, p, q, x);
             const double own = ((x[0] + x[1]) + x[2]) + x[3];
             double sum = own;
 #pragma unroll
@@ -285,7 +302,10 @@ __global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
 }  // namespace
 
 cudaError_t launch_verify(cudaStream_t st, const VerifyArgs& a) {
-    const int cluster = 8;
+    // blocks per request: enough to have about four on every SM (one request's row is then read by eight SMs), one for
+    // the larger batches, whose requests fill the GPU by themselves
+    int cluster = 8;
+    while (cluster > 1 && (int64_t)a.rows * cluster > 4 * 148) cluster >>= 1;
     return launch_serving(verify_kernel, dim3(a.rows * cluster), dim3(V_THREADS), 0, st, cluster, a);
 }
 
