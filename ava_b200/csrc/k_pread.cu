@@ -492,6 +492,9 @@ int64_t paged_read_workspace(int head_size, int sms) {
 }
 
 cudaError_t launch_paged_read(cudaStream_t st, const ReadArgs& a, void* room, int sms) {
+    bool taken = false;
+    const cudaError_t rc = launch_paged_read_tc(st, a, room, sms, &taken);
+    if (taken || rc != cudaSuccess) return rc;
     if (a.s.head_size == 32) return launch_size<32>(st, a, room, sms);
     if (a.s.head_size == 64) return launch_size<64>(st, a, room, sms);
     return launch_size<128>(st, a, room, sms);

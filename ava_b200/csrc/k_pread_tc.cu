@@ -1,0 +1,718 @@
+// The read of new tokens over a bf16 store in pages when a request brings many rows per key head (prompt chunks, drafted
+// runs with shared key heads): the same o = sum_j softmax_j(scale q . k_j) v_j on tcgen05 tensor cores.
+//
+// A block is a worker of read_split.cuh with tiles of 128 * QT rows and units of KT keys; its piece of the line is walked
+// stretch by stretch.  Per unit and 128-row tile: S = Q K^T into tensor memory (Q and K from shared memory), one thread per
+// row turns its row of S into weights with a running maximum and sum, and writes them over S as the bf16 operand of
+// O += P V (P from tensor memory, V from shared memory as it arrived, keys down: the multiply takes it that way).  O stays
+// in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8, so almost never after the first
+// units.  Two groups of 128 threads work on two tiles (QT 2) or on the odd and even units of one (QT 1): while one turns
+// its scores into weights the tensor cores multiply for the other.
+// Keys and values come by TMA, a box per page and 64 channels, into rings of their own; a page outside the store, or past
+// the stretch, is a coordinate past the tensor's last page, which TMA fills with zeros without reading.  Rows of V in
+// front of the stretch or behind it (the rest of a page, left padding) are written over with zeros in shared memory before
+// the multiply: a weight of 0 times whatever lies there must be 0.
+// With f32 queries Q and P are three bf16 limbs each (L 3): three products per step instead of one.
+//
+// S and P share their columns, so S of a tile's next unit waits for its P V; that wait is on the completion of the
+// multiply (multiplies into different accumulators are not ordered by their issue).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "ava_math.h"
+#include "bf16_hw.cuh"
+#include "kernels.cuh"
+#include "read_split.cuh"
+#include "serving.cuh"
+#include "tc_common.cuh"
+
+namespace ava {
+
+namespace {
+
+using namespace tcc;
+
+constexpr int THREADS = 384;             // two groups of 128 rows, the multiply's warp, the copies' warp (two more stand by:
+                                         // registers are given out by fours of warps)
+constexpr int ROW_REGS = 208, OTHER_REGS = 88;   // a thread's registers once the roles have split
+constexpr int LAUNCH_REGS = 168;         // what the launch has per thread: 65536 / 384, in eights
+static_assert(2 * ROW_REGS + OTHER_REGS <= 3 * LAUNCH_REGS, "the split draws on the launch's registers");
+constexpr int SNAP = 2;                  // stretches of up to this many units are not cut
+constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
+constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by before the sums are rescaled
+
+template <int HS_, int L_>
+struct Shape {
+    static constexpr int HS = HS_, L = L_;
+    static constexpr int KT = HS == 128 && L == 3 ? 64 : 128;        // keys per unit
+    static constexpr int QT = HS == 128 && L == 3 ? 1 : 2;           // 128-row tiles per block
+    static constexpr int MR = 128 * QT;
+    static constexpr int HALVES = HS / 64;                           // 64-channel columns of 128 bytes a row
+    static constexpr uint32_t Q_LIMB = 128 * HS * 2, Q_TILE = L * Q_LIMB, KV = KT * HS * 2;
+    static constexpr int NK = HS == 64 ? (L == 1 ? 5 : 3) : (L == 1 ? 3 : 4), NV = HS == 64 ? (L == 1 ? 5 : 3) : (L == 1 ? 2 : 4);
+    static constexpr uint32_t OFF_K = QT * Q_TILE, OFF_V = OFF_K + NK * KV, OFF_BAR = OFF_V + NV * KV, OFF_ML = OFF_BAR + 256;
+    static constexpr uint32_t BYTES = OFF_ML + (QT == 1 ? 1024 : 0) + 1024;   // the rest: alignment to 1024
+    // tensor memory of a group: scores (later the weights' first limbs), the third limb, the mix
+    static constexpr uint32_t C_LOW = KT, C_O = KT == 64 ? 128 : KT + (L == 3 ? KT / 2 : 0), C_GROUP = 256;
+    static_assert(C_O + HS <= C_GROUP, "tensor memory");
+    static_assert(BYTES <= 232448, "shared memory");
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float low_half(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float high_half(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+__device__ __forceinline__ void bar_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(bar)) : "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int page, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(page), "r"(s32(bar))
+                 : "memory");
+}
+// V as it lies, [key][64 channels] with the 128-byte swizzle, for a multiply that wants it [channel][key]: 64 channels
+// adjacent, 8 keys to 1024 bytes; `group` bytes from one 64-channel column to the next
+__device__ __forceinline__ uint64_t desc_keys_down(uint32_t at, uint32_t group) {
+    uint64_t d = 0;
+    d |= (uint64_t)((at & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(group >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+struct Bars {
+    uint64_t full_k[5], empty_k[5], full_v[5], empty_v[5], q_ready[2], s_ready[2], p_ready[2], pv_done[2], o_free[2];
+    uint32_t tmem, failed;
+};
+static_assert(sizeof(Bars) <= 256, "barriers");
+
+// A wait that ends: true when the phase is there, false when it ran out here or anywhere in the block.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
+    const uint32_t addr = s32(bar);
+    for (uint32_t i = 0; i < B_WAIT_LIMIT; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (i > 64) {
+            if (*failed) return false;
+            if (i > 1024) __nanosleep(32);
+        }
+    }
+    *failed = 1;
+    return false;
+}
+// the same answer for the whole warp
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
+    return __all_sync(0xffffffffu, wait(bar, parity, failed));
+}
+
+// A worker's run over one stretch: units [ta, tb) of the store's own KT-key units, and which of them each group works on.
+template <typename Sh>
+struct Run {
+    int ta, tb, rows;
+    int a[2], b[2];                      // QT 2: group w works on units [a, b); QT 1: on those of its parity in [ta, tb)
+    __device__ __forceinline__ bool has(int w, int t) const {
+        return Sh::QT == 2 ? t >= a[w] && t < b[w] : t >= ta && t < tb && ((t - ta) & 1) == w;
+    }
+    __device__ __forceinline__ int count(int w) const { return Sh::QT == 2 ? max(b[w] - a[w], 0) : (tb - ta + 1 - w) / 2; }
+    __device__ __forceinline__ int first(int w) const { return Sh::QT == 2 ? a[w] : ta + w; }
+};
+template <typename Sh>
+__device__ __forceinline__ Run<Sh> run_of(const ReadArgs& a, const split::Item& it, long long u, long long stop) {
+    Run<Sh> r;
+    const bool none = it.s.lo >= it.s.hi;
+    r.ta = none ? 0 : it.s.lo / Sh::KT + (int)(u - it.begin);
+    r.tb = none ? 0 : it.s.lo / Sh::KT + (int)(stop - it.begin);
+    r.rows = min(it.q.f * a.group - it.tile * Sh::MR, Sh::MR);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        r.a[w] = r.b[w] = r.ta;
+        if (Sh::QT == 2 && r.rows > 128 * w) {   // the keys that this tile's own rows see
+            const int m0 = it.tile * Sh::MR + 128 * w, m1 = it.tile * Sh::MR + min(r.rows, 128 * w + 128) - 1;
+            const int hi = it.q.c + m1 / a.group + 1, lo = a.window > 0 ? max(it.q.first, it.q.c + m0 / a.group + 1 - a.window) : it.q.first;
+            if (lo < hi) {
+                r.a[w] = max(r.ta, lo / Sh::KT);
+                r.b[w] = min(r.tb, (hi + Sh::KT - 1) / Sh::KT);
+            }
+        }
+    }
+    return r;
+}
+
+template <typename Sh>
+__global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ReadArgs a,
+                                                            const int heads_inside, const int box_rows, float* __restrict__ ends, split::Cut* __restrict__ cuts) {
+    constexpr int HS = Sh::HS, L = Sh::L, KT = Sh::KT, QT = Sh::QT, MR = Sh::MR;
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = raw + ((1024u - (s32(raw) & 1023u)) & 1023u);
+    const uint32_t at0 = s32(smem);
+    Bars* bars = reinterpret_cast<Bars*>(smem + Sh::OFF_BAR);
+    volatile uint32_t* failed = &bars->failed;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_enter();
+    // this block's piece of the line (the sums lie where the copies will)
+    bool bad_length = false;
+    const split::Line line = split::line<MR, KT>(a, reinterpret_cast<long long*>(smem + Sh::OFF_K), &bad_length);
+    if (bad_length && a.status && blockIdx.x == 0) atomicOr(a.status, AVA_PAGED_BAD_LENGTH);
+    const int worker = blockIdx.x;
+    const long long per = max((line.total() + gridDim.x - 1) / (long long)gridDim.x, 1ll);
+    split::Item it, after;
+    long long u = split::piece<MR, KT, SNAP>(a, line, per, worker, &it);
+    const long long end = split::piece<MR, KT, SNAP>(a, line, per, worker + 1ll, &after);
+    if (tid == 0) {
+        cuts[worker].workers = 0;
+        for (int i = 0; i < 5; ++i) {
+            bar_init(&bars->full_k[i], 1);
+            bar_init(&bars->empty_k[i], 1);
+            bar_init(&bars->full_v[i], 1);
+            bar_init(&bars->empty_v[i], 1);
+        }
+        for (int w = 0; w < 2; ++w) {
+            bar_init(&bars->q_ready[w], 128);
+            bar_init(&bars->s_ready[w], 1);
+            bar_init(&bars->p_ready[w], 128);
+            bar_init(&bars->pv_done[w], 1);
+            bar_init(&bars->o_free[w], 128);
+        }
+        bars->failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    fence_async();   // the sums were written where copies will be
+    __syncwarp();
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&bars->tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = bars->tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    bool ok = true;
+
+    if (warp < 8) {
+        // ---- one row per thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ROW_REGS));
+        const int w = warp >> 2, row = tid & 127, q_row = QT == 2 ? w * 128 + row : row;   // row within the block's tile
+        const uint32_t mine = tmem + w * Sh::C_GROUP + ((uint32_t)((warp & 3) * 32) << 16);
+        // the scale's sign goes into the queries, so that the largest score is the largest product
+        const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
+        const uint32_t q_sign = a.scale < 0.0f ? 0x80008000u : 0u, q_keep = a.scale == 0.0f ? 0u : 0xffffffffu;
+        const bool q_wide = !((reinterpret_cast<uintptr_t>(a.q) & 15) || (a.q_token_stride % (L == 3 ? 4 : 8)) || (a.q_head_stride % (L == 3 ? 4 : 8)));
+        const bool out_wide = !((reinterpret_cast<uintptr_t>(a.out) & 15) || (a.out_token_stride % (L == 3 ? 4 : 8)) || (a.out_head_stride % (L == 3 ? 4 : 8)));
+        uint32_t n_s = 0, n_pv = 0;      // units of this group so far: its barriers' phases
+        while (u < end && ok) {
+            const long long stop = min(end, it.begin + it.s.units);
+            const bool whole = u == it.begin && stop == it.begin + it.s.units;
+            const Run<Sh> run = run_of<Sh>(a, it, u, stop);
+            const int units = run.count(w);
+            const bool live = q_row < run.rows;
+            const int m = it.tile * MR + min(q_row, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
+            const int pos = it.q.c + i, low = a.window > 0 ? max(it.q.first, pos - a.window + 1) : it.q.first;
+            if (units > 0) {
+                // the query row into the operand layout (QT 1: the groups share one tile, the first writes it)
+                const int64_t from = (int64_t)(it.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride;
+                unsigned char* tile = smem + (QT == 2 ? w * Sh::Q_TILE : 0);
+                if (QT == 2 || w == 0) {
+#pragma unroll
+                    for (int c = 0; c < HS; c += 8) {
+                        const uint32_t to = (uint32_t)(c / 64) * (128 * 128) + swz128(row, c & 63);
+                        if constexpr (L == 3) {
+                            const float* q = static_cast<const float*>(a.q) + from + c;
+                            float x[8];
+                            if (q_wide) {
+                                const float4 y = *reinterpret_cast<const float4*>(q), z = *reinterpret_cast<const float4*>(q + 4);
+                                x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; x[4] = z.x; x[5] = z.y; x[6] = z.z; x[7] = z.w;
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) x[k] = q[k];
+                            }
+#pragma unroll
+                            for (int l = 0; l < L; ++l) {
+                                uint32_t p[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    p[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+                                    x[2 * k] = __fsub_rn(x[2 * k], low_half(p[k]));
+                                    x[2 * k + 1] = __fsub_rn(x[2 * k + 1], high_half(p[k]));
+                                }
+                                *reinterpret_cast<uint4*>(tile + l * Sh::Q_LIMB + to) = make_uint4((p[0] ^ q_sign) & q_keep, (p[1] ^ q_sign) & q_keep, (p[2] ^ q_sign) & q_keep, (p[3] ^ q_sign) & q_keep);
+                            }
+                        } else {
+                            const uint16_t* q = static_cast<const uint16_t*>(a.q) + from + c;
+                            uint4 p;
+                            if (q_wide) p = *reinterpret_cast<const uint4*>(q);
+                            else p = make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16), q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
+                            *reinterpret_cast<uint4*>(tile + to) = make_uint4((p.x ^ q_sign) & q_keep, (p.y ^ q_sign) & q_keep, (p.z ^ q_sign) & q_keep, (p.w ^ q_sign) & q_keep);
+                        }
+                    }
+                    fence_async();
+                }
+                bar_arrive(&bars->q_ready[w]);
+            }
+            float top = -INFINITY, sum = 0.0f;
+            for (int n = 0; n < units && ok; ++n) {
+                const int t = QT == 2 ? run.first(w) + n : run.first(w) + 2 * n;
+                ok = warp_wait(&bars->s_ready[w], n_s & 1, failed);
+                ++n_s;
+                if (!ok) break;
+                tc_after();
+                uint32_t s[KT];
+#pragma unroll
+                for (int c = 0; c < KT; c += 32) tmem_ld32(mine + c, s + c);
+                tmem_wait_ld();
+                const int from = low - t * KT, to = pos - t * KT;   // keys [from, to] of the unit are seen
+                if (__any_sync(0xffffffffu, from > 0 || to < KT - 1)) {
+#pragma unroll
+                    for (int j = 0; j < KT; ++j)
+                        if (j < from || j > to) s[j] = 0xff800000u;
+                }
+                float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < KT; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
+                const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
+                const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
+                    if (n > 0) {   // the unit before has been added up: its completion is what let these scores be made
+#pragma unroll
+                        for (int c = 0; c < HS; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(mine + Sh::C_O + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tmem_st16(mine + Sh::C_O + c, o);
+                            tmem_st16(mine + Sh::C_O + c + 16, o + 16);
+                        }
+                    }
+                    sum *= f;
+                    top = now;
+                }
+                const float base = top == -INFINITY ? 0.0f : top;
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < KT; c += 32) {   // 32 keys: 16 columns of weights per limb
+                    uint32_t p[L][16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float x = exp2_fast(fmaf(__uint_as_float(s[c + 2 * k]), scale2, -base));
+                        float y = exp2_fast(fmaf(__uint_as_float(s[c + 2 * k + 1]), scale2, -base));
+                        part[k & 1] += x;
+                        part[2 + (k & 1)] += y;
+#pragma unroll
+                        for (int l = 0; l < L; ++l) {
+                            p[l][k] = pack_bf16(x, y);
+                            x = __fsub_rn(x, low_half(p[l][k]));
+                            y = __fsub_rn(y, high_half(p[l][k]));
+                        }
+                    }
+#pragma unroll
+                    for (int l = 0; l < L; ++l) tmem_st16(mine + (l == 2 ? Sh::C_LOW : l * (KT / 2)) + c / 2, p[l]);
+                }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                tmem_wait_st();
+                tc_before();
+                bar_arrive(&bars->p_ready[w]);
+                ++n_pv;
+            }
+            // ---- the read of the row, or this piece's end of it
+            if (units > 0 && ok) ok = warp_wait(&bars->pv_done[w], (n_pv - 1) & 1, failed);
+            if (QT == 2 && !ok) break;
+            tc_after();
+            float other_f = 0.0f, own_f = 1.0f;
+            bool both = false;
+            if constexpr (QT == 1) {   // two groups hold parts of one row: the first joins them (their sums lie in the same lanes)
+                float* ml = reinterpret_cast<float*>(smem + Sh::OFF_ML);
+                if (w == 1) {
+                    ml[row] = top;
+                    ml[128 + row] = sum;
+                }
+                uint32_t off;   // one group's failed wait ends both: nobody is left at the barrier
+                asm volatile(
+                    "{\n\t.reg .pred p, q;\n\t"
+                    "setp.ne.u32 p, %1, 0;\n\t"
+                    "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+                    "selp.u32 %0, 1, 0, q;\n\t}"
+                    : "=r"(off)
+                    : "r"(ok ? 0u : 1u)
+                    : "memory");
+                ok = off == 0;
+                if (!ok) break;
+                if (w == 0) {
+                    const float t1 = ml[row], s1 = ml[128 + row], now = fmaxf(top, t1);
+                    own_f = top == -INFINITY ? 0.0f : exp2_fast(top - now);
+                    other_f = t1 == -INFINITY ? 0.0f : exp2_fast(t1 - now);
+                    sum = sum * own_f + s1 * other_f;
+                    top = now;
+                    both = run.count(1) > 0;
+                }
+            }
+            if (QT == 2 || w == 0) {
+                const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum) : 1.0f;
+                float* end_of = ends + ((int64_t)worker * 2 + (u == it.begin ? 1 : 0)) * (MR * (HS + 2));
+                const int64_t to = (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride;
+#pragma unroll
+                for (int c = 0; c < HS; c += 32) {
+                    uint32_t o[32];
+                    float x[32];
+                    if (units > 0) {
+                        tmem_ld32(mine + Sh::C_O + c, o);
+                        tmem_wait_ld();
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) x[k] = units > 0 ? __uint_as_float(o[k]) * own_f : 0.0f;
+                    if (QT == 1 && both) {
+                        tmem_ld32(mine + Sh::C_GROUP + Sh::C_O + c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) x[k] = fmaf(__uint_as_float(o[k]), other_f, x[k]);
+                    }
+                    if (!live) continue;
+                    if (!whole) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(end_of + q_row * HS + c + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+                    } else if constexpr (L == 3) {
+                        float* out = static_cast<float*>(a.out) + to + c;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            if (out_wide) *reinterpret_cast<float4*>(out + k) = make_float4(x[k] * inv, x[k + 1] * inv, x[k + 2] * inv, x[k + 3] * inv);
+                            else
+                                for (int y = 0; y < 4; ++y) out[k + y] = x[k + y] * inv;
+                        }
+                    } else {
+                        uint16_t* out = static_cast<uint16_t*>(a.out) + to + c;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            uint4 v;
+                            v.x = pack_bf16(x[k] * inv, x[k + 1] * inv);
+                            v.y = pack_bf16(x[k + 2] * inv, x[k + 3] * inv);
+                            v.z = pack_bf16(x[k + 4] * inv, x[k + 5] * inv);
+                            v.w = pack_bf16(x[k + 6] * inv, x[k + 7] * inv);
+                            if (out_wide) *reinterpret_cast<uint4*>(out + k) = v;
+                            else {
+                                const uint32_t y[4] = {v.x, v.y, v.z, v.w};
+                                for (int z = 0; z < 4; ++z) {
+                                    out[k + 2 * z] = (uint16_t)y[z];
+                                    out[k + 2 * z + 1] = (uint16_t)(y[z] >> 16);
+                                }
+                            }
+                        }
+                    }
+                }
+                if (live) {
+                    if (!whole) {
+                        end_of[MR * HS + q_row] = top;
+                        end_of[MR * HS + MR + q_row] = sum;
+                    } else if (a.lse) {
+                        a.lse[(int64_t)(it.q.start + i) * a.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * LN2;
+                    }
+                }
+                if (!whole && u == it.begin && tid == 0) {
+                    cuts[worker].r = it.r;
+                    cuts[worker].head = it.head;
+                    cuts[worker].tile = it.tile;
+                    cuts[worker].workers = (int)((it.begin + it.s.units - 1) / per) - worker + 1;
+                }
+            }
+            tc_before();
+            if constexpr (QT == 1) asm volatile("bar.sync 1, 256;" ::: "memory");   // the other group's sums have been read
+            if (units > 0) bar_arrive(&bars->o_free[w]);
+            u = stop;
+            if (u < end) split::next<MR, KT>(a, it);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    }
+    if (warp == 8) {
+        // ---- the multiplies: one thread issues, the warp clears the rows of V that belong to nobody
+        constexpr uint32_t i_s = instr_desc(KT), i_o = instr_desc(HS) | (1u << 16);   // V with its keys down
+        uint32_t tk = 0, tv = 0;                      // units loaded so far: the rings' places and phases
+        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};    // stretches and units of the groups so far
+        const bool one = lane == 0;
+        while (u < end && ok) {
+            const long long stop = min(end, it.begin + it.s.units);
+            const Run<Sh> run = run_of<Sh>(a, it, u, stop);
+            // unit t's scores for the groups that work on it, once what their columns held has been used up
+            auto scores = [&](int w, int t) {
+                if (t == run.first(w)) ok = ok && warp_wait(&bars->q_ready[w], n_q[w] & 1, failed);
+                if (n_p[w] > 0) ok = ok && warp_wait(&bars->pv_done[w], (n_p[w] - 1) & 1, failed);
+                const uint32_t slot = tk % Sh::NK;
+                ok = ok && warp_wait(&bars->full_k[slot], (tk / Sh::NK) & 1, failed);
+                if (ok && one) {
+                    tc_after();
+                    const unsigned char* q = smem + (QT == 2 ? w * Sh::Q_TILE : 0);
+                    const unsigned char* k = smem + Sh::OFF_K + slot * Sh::KV;
+#pragma unroll
+                    for (int l = 0; l < L; ++l)
+#pragma unroll
+                        for (int c = 0; c < HS / 16; ++c)
+                            mma_ss(tmem + w * Sh::C_GROUP, operand_desc(q + l * Sh::Q_LIMB + (c / 4) * (128 * 128)) + 2u * (c & 3),
+                                   operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l + c > 0);
+                    commit(&bars->s_ready[w]);
+                }
+                __syncwarp();
+            };
+            // the unit's keys are free once every group's scores are made (each unit of a run is some group's)
+            auto free_keys = [&]() {
+                if (ok && one) commit(&bars->empty_k[tk % Sh::NK]);
+                ++tk;
+            };
+            if (run.ta < run.tb) {
+                for (int w = 0; w < 2; ++w)
+                    if (run.has(w, run.ta)) scores(w, run.ta);
+                free_keys();
+            }
+            for (int t = run.ta; t < run.tb && ok; ++t) {
+                const uint32_t slot = tv % Sh::NV;
+                ok = warp_wait(&bars->full_v[slot], (tv / Sh::NV) & 1, failed);
+                if (!ok) break;
+                unsigned char* v = smem + Sh::OFF_V + slot * Sh::KV;
+                const int clear_to = it.s.lo - t * KT, clear_from = it.s.hi - t * KT;   // rows in front of the stretch, and behind it
+                if (clear_to > 0 || clear_from < KT) {
+                    for (int e = lane; e < KT * (HS / 8); e += 32) {
+                        const int key = e / (HS / 8), c = e % (HS / 8);
+                        if (key < clear_to || key >= clear_from) *reinterpret_cast<uint4*>(v + (c / 8) * (KT * 128) + swz128(key, (c & 7) * 8)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_async();
+                    __syncwarp();
+                }
+                for (int w = 0; w < 2 && ok; ++w) {
+                    if (run.has(w, t)) {
+                        ok = warp_wait(&bars->p_ready[w], n_p[w] & 1, failed);
+                        if (t == run.first(w) && n_q[w] > 0) ok = ok && warp_wait(&bars->o_free[w], (n_q[w] - 1) & 1, failed);
+                        if (!ok) break;
+                        if (one) {
+                            tc_after();
+                            const uint32_t p = tmem + w * Sh::C_GROUP;
+#pragma unroll
+                            for (int l = 0; l < L; ++l)
+#pragma unroll
+                                for (int c = 0; c < KT / 16; ++c)
+                                    mma_ts(p + Sh::C_O, p + (l == 2 ? Sh::C_LOW : l * (KT / 2)) + 8 * c, desc_keys_down(s32(v) + c * 2048, KT * 128), i_o,
+                                           t != run.first(w) || l + c > 0);
+                            commit(&bars->pv_done[w]);
+                        }
+                        __syncwarp();
+                        ++n_p[w];
+                        if (t == run.first(w)) ++n_q[w];
+                    }
+                    if (t + 1 < run.tb && run.has(w, t + 1)) scores(w, t + 1);
+                }
+                if (!ok) break;
+                if (t + 1 < run.tb) free_keys();
+                if (one) commit(&bars->empty_v[slot]);
+                ++tv;
+            }
+            u = stop;
+            if (u < end) split::next<MR, KT>(a, it);
+        }
+    } else if (warp == 9) {
+        // ---- the copies: a lane per box
+        uint32_t n = 0;
+        bool bad_page = false;
+        const int boxes = KT / box_rows * Sh::HALVES;
+        while (u < end && ok) {
+            const long long stop = min(end, it.begin + it.s.units);
+            const Run<Sh> run = run_of<Sh>(a, it, u, stop);
+            const int32_t* pages = a.table + (int64_t)it.r * a.max_pages;
+            for (int t = run.ta; t < run.tb && ok; ++t, ++n) {
+                // a box is box_rows keys of one page (a unit's keys may lie within one page or run over several)
+                int page = a.s.n_pages, place = 0;
+                const int b = lane % (KT / box_rows), j = t * KT + b * box_rows;
+                if (lane < boxes && j < it.s.hi && j + box_rows > it.s.lo) {
+                    const int pi = j / a.s.page_size;
+                    page = pages[pi];
+                    place = j - pi * a.s.page_size;
+                    if (page < 0 || page >= a.s.n_pages) {
+                        bad_page = true;
+                        page = a.s.n_pages;
+                    }
+                }
+#pragma unroll
+                for (int kv = 0; kv < 2 && ok; ++kv) {
+                    const uint32_t ring = kv ? Sh::NV : Sh::NK, slot = n % ring, turn = n / ring;
+                    uint64_t* full = kv ? &bars->full_v[slot] : &bars->full_k[slot];
+                    uint64_t* empty = kv ? &bars->empty_v[slot] : &bars->empty_k[slot];
+                    if (turn > 0) ok = warp_wait(empty, (turn - 1) & 1, failed);
+                    if (!ok) break;
+                    if (lane == 0) bar_expect(full, Sh::KV);
+                    __syncwarp();
+                    const uint32_t dst = at0 + (kv ? Sh::OFF_V : Sh::OFF_K) + slot * Sh::KV;
+                    if (lane < boxes) {   // at most 32: boxes of 8 keys and more
+                        const int half = lane / (KT / box_rows);
+                        tma_box(dst + half * (KT * 128) + b * box_rows * 128, kv ? &map_v : &map_k, half * 64, heads_inside ? it.head : place,
+                                heads_inside ? place : it.head, page, full);
+                    }
+                    __syncwarp();
+                }
+            }
+            u = stop;
+            if (u < end) split::next<MR, KT>(a, it);
+        }
+        if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
+        if (!ok) {   // the copies in flight end before the block does
+            for (uint32_t back = 1; back <= 5; ++back) {
+                if (n >= back && back <= Sh::NK) bar_wait(&bars->full_k[(n - back) % Sh::NK], ((n - back) / Sh::NK) & 1);
+                if (n >= back && back <= Sh::NV) bar_wait(&bars->full_v[(n - back) % Sh::NV], ((n - back) / Sh::NV) & 1);
+            }
+        }
+    }
+    if (!ok && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_WAIT_RAN_OUT);
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// Joins the ends of the stretches that were cut (see k_pread.cu): a block per worker and eight rows, a warp per row.
+template <int HS, int MR>
+__global__ void __launch_bounds__(256) join_rows_kernel(const ReadArgs a, const float* __restrict__ ends, const split::Cut* __restrict__ cuts) {
+    pdl_enter();
+    const int w = blockIdx.x, n = cuts[w].workers, lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (n == 0) return;
+    constexpr int PER = HS / 32;
+    bool bad = false;
+    const split::Request q = split::request(a, cuts[w].r, &bad);
+    const int head = cuts[w].head, tile = cuts[w].tile;
+    if (row >= min(q.f * a.group - tile * MR, MR)) return;
+    float m = -INFINITY, l = 0.0f, o[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = 0.0f;
+    for (int k = 0; k < n; ++k) {
+        const float* part = ends + ((int64_t)(w + k) * 2 + (k == 0 ? 1 : 0)) * (MR * (HS + 2));
+        const float mk = part[MR * HS + row], lk = part[MR * HS + MR + row], mn = fmaxf(m, mk);
+        const float fo = m == -INFINITY ? 0.0f : exp2_fast(m - mn), fk = mk == -INFINITY ? 0.0f : exp2_fast(mk - mn);
+        l = l * fo + lk * fk;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) o[i] = o[i] * fo + part[row * HS + lane + 32 * i] * fk;
+        m = mn;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : l;
+    const int mm = tile * MR + row, i = mm / a.group, h = head * a.group + (mm - i * a.group);
+    const int64_t to = (int64_t)(q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride + lane;
+#pragma unroll
+    for (int c = 0; c < PER; ++c) {
+        if (a.bf16_q) static_cast<uint16_t*>(a.out)[to + 32 * c] = bf16_rn_hw(o[c] * inv);
+        else static_cast<float*>(a.out)[to + 32 * c] = o[c] * inv;
+    }
+    if (a.lse && lane == 0) a.lse[(int64_t)(q.start + i) * a.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// A pool as a tensor of [pages][...][...][channels] with the smaller of the head and place strides inside, as long as the
+// strides nest (each a multiple of the one inside it and at least its extent): what a tensor map describes.
+struct Pool {
+    bool heads_inside;
+    uint64_t dims[4], strides[3];
+};
+bool nested(const ava_paged_store& s, Pool* p) {
+    p->heads_inside = s.head_stride <= s.place_stride;
+    const int64_t n1 = p->heads_inside ? s.kv_heads : s.page_size, n2 = p->heads_inside ? s.page_size : s.kv_heads;
+    int64_t s1 = p->heads_inside ? s.head_stride : s.place_stride, s2 = p->heads_inside ? s.place_stride : s.head_stride, s3 = s.page_stride;
+    if (n1 == 1) s1 = s.head_size;     // the stride of a single head or place says nothing
+    if (n2 == 1) s2 = n1 * s1;
+    if (s.n_pages == 1) s3 = n2 * s2;
+    if (s1 < s.head_size || s1 % 8 || s2 < n1 * s1 || s2 % s1 || s3 < n2 * s2 || s3 % s2 || s3 >= (1ll << 39)) return false;
+    const uint64_t d[4] = {(uint64_t)s.head_size, (uint64_t)n1, (uint64_t)n2, (uint64_t)s.n_pages};
+    for (int i = 0; i < 4; ++i) p->dims[i] = d[i];
+    p->strides[0] = (uint64_t)s1 * 2;
+    p->strides[1] = (uint64_t)s2 * 2;
+    p->strides[2] = (uint64_t)s3 * 2;
+    return true;
+}
+bool pool_map(CUtensorMap* map, const void* base, const Pool& p, uint32_t box_rows) {
+    EncodeFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {p.dims[0], p.dims[1], p.dims[2], p.dims[3]}, strides[3] = {p.strides[0], p.strides[1], p.strides[2]};
+    const cuuint32_t box[4] = {64, p.heads_inside ? 1u : box_rows, p.heads_inside ? box_rows : 1u, 1}, es[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HS, int L>
+cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, const Pool& pool, bool* taken) {
+    using Sh = Shape<HS, L>;
+    const int box_rows = a.s.page_size < Sh::KT ? a.s.page_size : Sh::KT;
+    if (box_rows < 8 || Sh::KT % box_rows || a.s.page_size % box_rows) return cudaSuccess;
+    CUtensorMap mk, mv;
+    if (!pool_map(&mk, a.s.k, pool, (uint32_t)box_rows) || !pool_map(&mv, a.s.v, pool, (uint32_t)box_rows)) return cudaSuccess;
+    cudaFuncAttributes attr;   // a split of registers beyond the launch's would never be granted
+    cudaError_t rc = cudaFuncGetAttributes(&attr, read_tc_kernel<Sh>);
+    if (rc != cudaSuccess) return rc;
+    if (attr.numRegs < LAUNCH_REGS) return cudaSuccess;
+    *taken = true;
+    split::Cut* cuts = static_cast<split::Cut*>(room);
+    float* ends = reinterpret_cast<float*>(cuts + sms);
+    rc = launch_serving(read_tc_kernel<Sh>, dim3(sms), dim3(THREADS), Sh::BYTES, st, 1, mk, mv, a, pool.heads_inside ? 1 : 0, box_rows, ends, cuts);
+    if (rc != cudaSuccess) return rc;
+    return launch_serving(join_rows_kernel<HS, Sh::MR>, dim3(sms, Sh::MR / 8), dim3(256), 0, st, 1, a, ends, cuts);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_read_tc(cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken) {
+    *taken = false;
+    Pool pool;
+    if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && a.s.head_size != 128) || (int64_t)a.max_fresh * a.group <= 32 || !nested(a.s, &pool)) return cudaSuccess;
+    if (a.s.head_size == 64) return a.bf16_q ? launch_one<64, 1>(st, a, room, sms, pool, taken) : launch_one<64, 3>(st, a, room, sms, pool, taken);
+    return a.bf16_q ? launch_one<128, 1>(st, a, room, sms, pool, taken) : launch_one<128, 3>(st, a, room, sms, pool, taken);
+}
+
+}  // namespace ava

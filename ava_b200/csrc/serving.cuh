@@ -70,6 +70,8 @@ struct ReadArgs {
 // room: paged_read_workspace bytes
 cudaError_t launch_paged_read(cudaStream_t st, const ReadArgs& a, void* room, int sms);
 int64_t paged_read_workspace(int head_size, int sms);
+// the same on tcgen05 (k_pread_tc.cu); *taken false: not its case, nothing was queued
+cudaError_t launch_paged_read_tc(cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken);
 
 // ---- drafted tokens (k_verify.cu)
 struct VerifyArgs {

@@ -10,7 +10,7 @@ step, src/diary.rs:686-718).  Every tensor lives on one CUDA device and is the c
 waited for, the work is queued on the device's current stream (or `stream`, a cudaStream_t as an int) and may be captured
 into a CUDA graph.  Tensors of a wrong type, shape or device raise ValueError, what the library refuses EngineError or
 NotApplicable; what only the GPU can see is ORed into `status` (an int32 or uint32 tensor of one element): the bits
-NO_PAGES to NO_MASS below.
+NO_PAGES to WAIT_RAN_OUT below.
 """
 from __future__ import annotations
 
@@ -20,7 +20,7 @@ import torch
 
 from . import engine
 
-NO_PAGES, NO_TABLE, BAD_LENGTH, NO_TOKENS, BAD_PAGE, BAD_TOKEN, NO_MASS = 1, 2, 4, 8, 16, 32, 64
+NO_PAGES, NO_TABLE, BAD_LENGTH, NO_TOKENS, BAD_PAGE, BAD_TOKEN, NO_MASS, WAIT_RAN_OUT = 1, 2, 4, 8, 16, 32, 64, 128
 NO_TOKEN = 0xFFFFFFFF   # -1 in an int32 tensor
 
 _I32, _I64, _F32, _F64, _BF16 = torch.int32, torch.int64, torch.float32, torch.float64, torch.bfloat16

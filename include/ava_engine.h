@@ -502,6 +502,7 @@ int ava_debug_mem_heads_wait_runs_out(int device, int32_t m, int32_t hs, int32_t
 #define AVA_PAGED_BAD_PAGE 16u     /* a page or slot outside the store */
 #define AVA_PAGED_BAD_TOKEN 32u    /* a drafted token outside the vocabulary */
 #define AVA_PAGED_NO_MASS 64u      /* probabilities that sum to nothing, or not to a finite number */
+#define AVA_PAGED_WAIT_RAN_OUT 128u /* a bounded wait inside a kernel ran out: what that call wrote is not to be used */
 #define AVA_NO_TOKEN 0xffffffffu
 /* Text of the last argument or launch error of these calls on this thread (never NULL). */
 const char* ava_serving_last_error(void);
