@@ -32,11 +32,7 @@ namespace {
 
 using namespace tcc;
 
-constexpr int THREADS = 384;             // two groups of 128 rows, the multiply's warp, the copies' warp (two more stand by:
-                                         // registers are given out by fours of warps)
-constexpr int ROW_REGS = 208, OTHER_REGS = 88;   // a thread's registers once the roles have split
-constexpr int LAUNCH_REGS = 168;         // what the launch has per thread: 65536 / 384, in eights
-static_assert(2 * ROW_REGS + OTHER_REGS <= 3 * LAUNCH_REGS, "the split draws on the launch's registers");
+constexpr int THREADS = 384;             // two groups of 128 rows, the multiply's warp, the copies' warp, the queries' two
 constexpr int SNAP = 2;                  // stretches of up to this many units are not cut
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by before the sums are rescaled
@@ -50,10 +46,12 @@ struct Shape {
     static constexpr int HALVES = HS / 64;                           // 64-channel columns of 128 bytes a row
     static constexpr uint32_t Q_LIMB = 128 * HS * 2, Q_TILE = L * Q_LIMB, KV = KT * HS * 2;
     static constexpr int NK = HS == 64 ? (L == 1 ? 5 : 3) : (L == 1 ? 3 : 4), NV = HS == 64 ? (L == 1 ? 5 : 3) : (L == 1 ? 2 : 4);
-    static constexpr uint32_t OFF_K = QT * Q_TILE, OFF_V = OFF_K + NK * KV, OFF_BAR = OFF_V + NV * KV, OFF_ML = OFF_BAR + 256;
+    static constexpr uint32_t OFF_K = QT * Q_TILE, OFF_V = OFF_K + NK * KV, OFF_BAR = OFF_V + NV * KV, OFF_ML = OFF_BAR + 512;
     static constexpr uint32_t BYTES = OFF_ML + (QT == 1 ? 1024 : 0) + 1024;   // the rest: alignment to 1024
-    // tensor memory of a group: scores (later the weights' first limbs), the third limb, the mix
-    static constexpr uint32_t C_LOW = KT, C_O = KT == 64 ? 128 : KT + (L == 3 ? KT / 2 : 0), C_GROUP = 256;
+    // Tensor memory of a group: the scores, the weights' third limbs, the mix.  A stretch of 32 scores is read at once and
+    // its weights go back over it: the first limb in its first 16 columns, the second in its last 16, the third outside.
+    static __device__ __forceinline__ uint32_t weights_at(int l, int c) { return l == 2 ? KT + c / 2 : c + 16 * l; }   // of keys c .. c + 31
+    static constexpr uint32_t C_O = KT == 64 ? 128 : KT + (L == 3 ? KT / 2 : 0), C_GROUP = 256;
     static_assert(C_O + HS <= C_GROUP, "tensor memory");
     static_assert(BYTES <= 232448, "shared memory");
 };
@@ -70,6 +68,31 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ float low_half(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high_half(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void apart(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// the next limb of a pair: bf16 of it, and what that leaves over
+__device__ __forceinline__ uint32_t limb(uint64_t& x) {
+    float a, b;
+    apart(x, a, b);
+    const uint32_t p = pack_bf16(a, b);
+    x = fma2(two(low_half(p), high_half(p)), two(-1.0f, -1.0f), x);
+    return p;
+}
 __device__ __forceinline__ void bar_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(bar)) : "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -132,10 +155,10 @@ __device__ __forceinline__ uint64_t desc_keys_down(uint32_t at, uint32_t group) 
 }
 
 struct Bars {
-    uint64_t full_k[5], empty_k[5], full_v[5], empty_v[5], q_ready[2], s_ready[2], p_ready[2], pv_done[2], o_free[2];
+    uint64_t full_k[5], empty_k[5], full_v[5], empty_v[5], q_ready[2], q_free[2], s_ready[2], p_ready[2], pv_done[2], o_free[2];
     uint32_t tmem, failed;
 };
-static_assert(sizeof(Bars) <= 256, "barriers");
+static_assert(sizeof(Bars) <= 512, "barriers");
 
 // A wait that ends: true when the phase is there, false when it ran out here or anywhere in the block.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
@@ -225,7 +248,8 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             bar_init(&bars->empty_v[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
-            bar_init(&bars->q_ready[w], 128);
+            bar_init(&bars->q_ready[w], QT == 2 ? 1 : 2);   // the warps that bring a tile of queries
+            bar_init(&bars->q_free[w], 1);
             bar_init(&bars->s_ready[w], 1);
             bar_init(&bars->p_ready[w], 128);
             bar_init(&bars->pv_done[w], 1);
@@ -249,13 +273,9 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
 
     if (warp < 8) {
         // ---- one row per thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ROW_REGS));
         const int w = warp >> 2, row = tid & 127, q_row = QT == 2 ? w * 128 + row : row;   // row within the block's tile
         const uint32_t mine = tmem + w * Sh::C_GROUP + ((uint32_t)((warp & 3) * 32) << 16);
-        // the scale's sign goes into the queries, so that the largest score is the largest product
-        const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
-        const uint32_t q_sign = a.scale < 0.0f ? 0x80008000u : 0u, q_keep = a.scale == 0.0f ? 0u : 0xffffffffu;
-        const bool q_wide = !((reinterpret_cast<uintptr_t>(a.q) & 15) || (a.q_token_stride % (L == 3 ? 4 : 8)) || (a.q_head_stride % (L == 3 ? 4 : 8)));
+        const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;   // its sign is in the queries
         const bool out_wide = !((reinterpret_cast<uintptr_t>(a.out) & 15) || (a.out_token_stride % (L == 3 ? 4 : 8)) || (a.out_head_stride % (L == 3 ? 4 : 8)));
         uint32_t n_s = 0, n_pv = 0;      // units of this group so far: its barriers' phases
         while (u < end && ok) {
@@ -266,47 +286,6 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             const bool live = q_row < run.rows;
             const int m = it.tile * MR + min(q_row, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
             const int pos = it.q.c + i, low = a.window > 0 ? max(it.q.first, pos - a.window + 1) : it.q.first;
-            if (units > 0) {
-                // the query row into the operand layout (QT 1: the groups share one tile, the first writes it)
-                const int64_t from = (int64_t)(it.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride;
-                unsigned char* tile = smem + (QT == 2 ? w * Sh::Q_TILE : 0);
-                if (QT == 2 || w == 0) {
-#pragma unroll
-                    for (int c = 0; c < HS; c += 8) {
-                        const uint32_t to = (uint32_t)(c / 64) * (128 * 128) + swz128(row, c & 63);
-                        if constexpr (L == 3) {
-                            const float* q = static_cast<const float*>(a.q) + from + c;
-                            float x[8];
-                            if (q_wide) {
-                                const float4 y = *reinterpret_cast<const float4*>(q), z = *reinterpret_cast<const float4*>(q + 4);
-                                x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; x[4] = z.x; x[5] = z.y; x[6] = z.z; x[7] = z.w;
-                            } else {
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) x[k] = q[k];
-                            }
-#pragma unroll
-                            for (int l = 0; l < L; ++l) {
-                                uint32_t p[4];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    p[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
-                                    x[2 * k] = __fsub_rn(x[2 * k], low_half(p[k]));
-                                    x[2 * k + 1] = __fsub_rn(x[2 * k + 1], high_half(p[k]));
-                                }
-                                *reinterpret_cast<uint4*>(tile + l * Sh::Q_LIMB + to) = make_uint4((p[0] ^ q_sign) & q_keep, (p[1] ^ q_sign) & q_keep, (p[2] ^ q_sign) & q_keep, (p[3] ^ q_sign) & q_keep);
-                            }
-                        } else {
-                            const uint16_t* q = static_cast<const uint16_t*>(a.q) + from + c;
-                            uint4 p;
-                            if (q_wide) p = *reinterpret_cast<const uint4*>(q);
-                            else p = make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16), q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
-                            *reinterpret_cast<uint4*>(tile + to) = make_uint4((p.x ^ q_sign) & q_keep, (p.y ^ q_sign) & q_keep, (p.z ^ q_sign) & q_keep, (p.w ^ q_sign) & q_keep);
-                        }
-                    }
-                    fence_async();
-                }
-                bar_arrive(&bars->q_ready[w]);
-            }
             float top = -INFINITY, sum = 0.0f;
             for (int n = 0; n < units && ok; ++n) {
                 const int t = QT == 2 ? run.first(w) + n : run.first(w) + 2 * n;
@@ -314,25 +293,30 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 ++n_s;
                 if (!ok) break;
                 tc_after();
-                uint32_t s[KT];
-#pragma unroll
-                for (int c = 0; c < KT; c += 32) tmem_ld32(mine + c, s + c);
-                tmem_wait_ld();
+                // Both passes over the row go 32 columns at a time, in loops that are not unrolled: straight through, the
+                // code was larger than the instruction caches keep at hand and half the time went into fetching it.
                 const int from = low - t * KT, to = pos - t * KT;   // keys [from, to] of the unit are seen
-                if (__any_sync(0xffffffffu, from > 0 || to < KT - 1)) {
-#pragma unroll
-                    for (int j = 0; j < KT; ++j)
-                        if (j < from || j > to) s[j] = 0xff800000u;
-                }
+                const bool edge = __any_sync(0xffffffffu, from > 0 || to < KT - 1);
                 float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int c = 0; c < KT; c += 32) {
+                    uint32_t s[32];
+                    tmem_ld32(mine + c, s);
+                    tmem_wait_ld();
+                    if (edge) {
 #pragma unroll
-                for (int j = 0; j < KT; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
+                        for (int j = 0; j < 32; ++j)
+                            if (c + j < from || c + j > to) s[j] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
+                }
                 const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
                 const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
                 if (__any_sync(0xffffffffu, grown)) {
                     const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
                     if (n > 0) {   // the unit before has been added up: its completion is what let these scores be made
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < HS; c += 32) {
                             uint32_t o[32];
                             tmem_ld32(mine + Sh::C_O + c, o);
@@ -347,27 +331,39 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     top = now;
                 }
                 const float base = top == -INFINITY ? 0.0f : top;
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t scales = two(scale2, scale2), bases = two(-base, -base);
+                uint64_t part[2] = {0ull, 0ull};
+#pragma unroll 1
+                for (int c = 0; c < KT; c += 32) {
+                    uint32_t s[32], p[L][16];
+                    tmem_ld32(mine + c, s);
+                    tmem_wait_ld();
+                    if (edge) {
 #pragma unroll
-                for (int c = 0; c < KT; c += 32) {   // 32 keys: 16 columns of weights per limb
-                    uint32_t p[L][16];
+                        for (int j = 0; j < 32; ++j)
+                            if (c + j < from || c + j > to) s[j] = 0xff800000u;
+                    }
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        float x = exp2_fast(fmaf(__uint_as_float(s[c + 2 * k]), scale2, -base));
-                        float y = exp2_fast(fmaf(__uint_as_float(s[c + 2 * k + 1]), scale2, -base));
-                        part[k & 1] += x;
-                        part[2 + (k & 1)] += y;
+                        float x, y;
+                        apart(fma2(two(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scales, bases), x, y);
+                        x = exp2_fast(x);
+                        y = exp2_fast(y);
+                        uint64_t e = two(x, y);
+                        part[k & 1] = add2(part[k & 1], e);
+                        if constexpr (L == 1) {
+                            p[0][k] = pack_bf16(x, y);
+                        } else {
 #pragma unroll
-                        for (int l = 0; l < L; ++l) {
-                            p[l][k] = pack_bf16(x, y);
-                            x = __fsub_rn(x, low_half(p[l][k]));
-                            y = __fsub_rn(y, high_half(p[l][k]));
+                            for (int l = 0; l < L; ++l) p[l][k] = limb(e);
                         }
                     }
 #pragma unroll
-                    for (int l = 0; l < L; ++l) tmem_st16(mine + (l == 2 ? Sh::C_LOW : l * (KT / 2)) + c / 2, p[l]);
+                    for (int l = 0; l < L; ++l) tmem_st16(mine + Sh::weights_at(l, c), p[l]);
                 }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                float x, y;
+                apart(add2(part[0], part[1]), x, y);
+                sum += x + y;
                 tmem_wait_st();
                 tc_before();
                 bar_arrive(&bars->p_ready[w]);
@@ -409,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum) : 1.0f;
                 float* end_of = ends + ((int64_t)worker * 2 + (u == it.begin ? 1 : 0)) * (MR * (HS + 2));
                 const int64_t to = (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < HS; c += 32) {
                     uint32_t o[32];
                     float x[32];
@@ -478,27 +474,28 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
         }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-    }
-    if (warp == 8) {
+    } else if (warp == 8) {
         // ---- the multiplies: one thread issues, the warp clears the rows of V that belong to nobody
         constexpr uint32_t i_s = instr_desc(KT), i_o = instr_desc(HS) | (1u << 16);   // V with its keys down
         uint32_t tk = 0, tv = 0;                      // units loaded so far: the rings' places and phases
-        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};    // stretches and units of the groups so far
+        uint32_t n_q[2] = {0, 0}, n_o[2] = {0, 0}, n_p[2] = {0, 0};   // tiles of queries, stretches and units of the groups so far
         const bool one = lane == 0;
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
             const Run<Sh> run = run_of<Sh>(a, it, u, stop);
             // unit t's scores for the groups that work on it, once what their columns held has been used up
             auto scores = [&](int w, int t) {
-                if (t == run.first(w)) ok = ok && warp_wait(&bars->q_ready[w], n_q[w] & 1, failed);
+                const int tile = QT == 2 ? w : 0;
+                if (t == run.first(w) && (QT == 2 || w == 0)) {
+                    ok = ok && warp_wait(&bars->q_ready[tile], n_q[tile] & 1, failed);
+                    ++n_q[tile];
+                }
                 if (n_p[w] > 0) ok = ok && warp_wait(&bars->pv_done[w], (n_p[w] - 1) & 1, failed);
                 const uint32_t slot = tk % Sh::NK;
                 ok = ok && warp_wait(&bars->full_k[slot], (tk / Sh::NK) & 1, failed);
                 if (ok && one) {
                     tc_after();
-                    const unsigned char* q = smem + (QT == 2 ? w * Sh::Q_TILE : 0);
+                    const unsigned char* q = smem + tile * Sh::Q_TILE;
                     const unsigned char* k = smem + Sh::OFF_K + slot * Sh::KV;
 #pragma unroll
                     for (int l = 0; l < L; ++l)
@@ -507,6 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                             mma_ss(tmem + w * Sh::C_GROUP, operand_desc(q + l * Sh::Q_LIMB + (c / 4) * (128 * 128)) + 2u * (c & 3),
                                    operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l + c > 0);
                     commit(&bars->s_ready[w]);
+                    if (t == (QT == 2 ? run.b[w] : run.tb) - 1) commit(&bars->q_free[tile]);   // the stretch's last scores of this tile
                 }
                 __syncwarp();
             };
@@ -537,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 for (int w = 0; w < 2 && ok; ++w) {
                     if (run.has(w, t)) {
                         ok = warp_wait(&bars->p_ready[w], n_p[w] & 1, failed);
-                        if (t == run.first(w) && n_q[w] > 0) ok = ok && warp_wait(&bars->o_free[w], (n_q[w] - 1) & 1, failed);
+                        if (t == run.first(w) && n_o[w] > 0) ok = ok && warp_wait(&bars->o_free[w], (n_o[w] - 1) & 1, failed);
                         if (!ok) break;
                         if (one) {
                             tc_after();
@@ -546,13 +544,13 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                             for (int l = 0; l < L; ++l)
 #pragma unroll
                                 for (int c = 0; c < KT / 16; ++c)
-                                    mma_ts(p + Sh::C_O, p + (l == 2 ? Sh::C_LOW : l * (KT / 2)) + 8 * c, desc_keys_down(s32(v) + c * 2048, KT * 128), i_o,
+                                    mma_ts(p + Sh::C_O, p + Sh::weights_at(l, c / 2 * 32) + 8 * (c & 1), desc_keys_down(s32(v) + c * 2048, KT * 128), i_o,
                                            t != run.first(w) || l + c > 0);
                             commit(&bars->pv_done[w]);
                         }
                         __syncwarp();
                         ++n_p[w];
-                        if (t == run.first(w)) ++n_q[w];
+                        if (t == run.first(w)) ++n_o[w];
                     }
                     if (t + 1 < run.tb && run.has(w, t + 1)) scores(w, t + 1);
                 }
@@ -613,6 +611,63 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 if (n >= back && back <= Sh::NK) bar_wait(&bars->full_k[(n - back) % Sh::NK], ((n - back) / Sh::NK) & 1);
                 if (n >= back && back <= Sh::NV) bar_wait(&bars->full_v[(n - back) % Sh::NV], ((n - back) / Sh::NV) & 1);
             }
+        }
+    } else if (warp >= 10) {
+        // ---- the queries of the next stretch, while this one's weights are still being made: a warp per tile (QT 1: half of
+        // the tile's rows each) into the operand layout, eight pieces of a row's channels in flight per lane
+        constexpr int CH = L == 3 ? 4 : 8, PIECES = HS / CH, ROWS = QT == 2 ? 128 : 64, AT_ONCE = 8;
+        const int tile = QT == 2 ? warp - 10 : 0, row0 = QT == 2 ? 0 : (warp - 10) * 64;
+        const bool wide = !((reinterpret_cast<uintptr_t>(a.q) & 15) || (a.q_token_stride % CH) || (a.q_head_stride % CH));
+        // the scale's sign goes into the queries, so that the largest score is the largest product; a scale of 0 empties them
+        const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
+        unsigned char* to = smem + tile * Sh::Q_TILE;
+        uint32_t n = 0;
+        while (u < end && ok) {
+            const long long stop = min(end, it.begin + it.s.units);
+            const Run<Sh> run = run_of<Sh>(a, it, u, stop);
+            if (QT == 2 ? run.count(tile) > 0 : run.ta < run.tb) {
+                if (n > 0) ok = warp_wait(&bars->q_free[tile], (n - 1) & 1, failed);
+                if (!ok) break;
+                ++n;
+                for (int e0 = 0; e0 < ROWS * PIECES; e0 += 32 * AT_ONCE) {
+                    uint4 x[AT_ONCE];
+#pragma unroll
+                    for (int k = 0; k < AT_ONCE; ++k) {
+                        const int e = e0 + k * 32 + lane, c = (e % PIECES) * CH;
+                        const int m = it.tile * MR + min(tile * 128 + row0 + e / PIECES, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
+                        const int64_t from = (int64_t)(it.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride + c;
+                        if (wide) {
+                            x[k] = *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) + from * (L == 3 ? 4 : 2));
+                        } else if (L == 3) {
+                            const uint32_t* q = static_cast<const uint32_t*>(a.q) + from;
+                            x[k] = make_uint4(q[0], q[1], q[2], q[3]);
+                        } else {
+                            const uint16_t* q = static_cast<const uint16_t*>(a.q) + from;
+                            x[k] = make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16), q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < AT_ONCE; ++k) {
+                        const int e = e0 + k * 32 + lane, c = (e % PIECES) * CH;
+                        unsigned char* at = to + (c / 64) * (128 * 128) + swz128(row0 + e / PIECES, c & 63);
+                        if constexpr (L == 3) {
+                            uint64_t y = two(__uint_as_float(x[k].x), __uint_as_float(x[k].y)), z = two(__uint_as_float(x[k].z), __uint_as_float(x[k].w));
+#pragma unroll
+                            for (int l = 0; l < L; ++l) {
+                                const uint32_t v = limb(y), w = limb(z);
+                                *reinterpret_cast<uint2*>(at + l * Sh::Q_LIMB) = make_uint2((v ^ sign) & keep, (w ^ sign) & keep);
+                            }
+                        } else {
+                            *reinterpret_cast<uint4*>(at) = make_uint4((x[k].x ^ sign) & keep, (x[k].y ^ sign) & keep, (x[k].z ^ sign) & keep, (x[k].w ^ sign) & keep);
+                        }
+                    }
+                }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars->q_ready[tile]);
+            }
+            u = stop;
+            if (u < end) split::next<MR, KT>(a, it);
         }
     }
     if (!ok && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_WAIT_RAN_OUT);
@@ -693,14 +748,10 @@ cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, 
     if (box_rows < 8 || Sh::KT % box_rows || a.s.page_size % box_rows) return cudaSuccess;
     CUtensorMap mk, mv;
     if (!pool_map(&mk, a.s.k, pool, (uint32_t)box_rows) || !pool_map(&mv, a.s.v, pool, (uint32_t)box_rows)) return cudaSuccess;
-    cudaFuncAttributes attr;   // a split of registers beyond the launch's would never be granted
-    cudaError_t rc = cudaFuncGetAttributes(&attr, read_tc_kernel<Sh>);
-    if (rc != cudaSuccess) return rc;
-    if (attr.numRegs < LAUNCH_REGS) return cudaSuccess;
     *taken = true;
     split::Cut* cuts = static_cast<split::Cut*>(room);
     float* ends = reinterpret_cast<float*>(cuts + sms);
-    rc = launch_serving(read_tc_kernel<Sh>, dim3(sms), dim3(THREADS), Sh::BYTES, st, 1, mk, mv, a, pool.heads_inside ? 1 : 0, box_rows, ends, cuts);
+    cudaError_t rc = launch_serving(read_tc_kernel<Sh>, dim3(sms), dim3(THREADS), Sh::BYTES, st, 1, mk, mv, a, pool.heads_inside ? 1 : 0, box_rows, ends, cuts);
     if (rc != cudaSuccess) return rc;
     return launch_serving(join_rows_kernel<HS, Sh::MR>, dim3(sms, Sh::MR / 8), dim3(256), 0, st, 1, a, ends, cuts);
 }
