@@ -14,8 +14,10 @@
 // the multiply: a weight of 0 times whatever lies there must be 0.
 // With f32 queries Q and P are three bf16 limbs each (L 3): three products per step instead of one.
 //
-// S and P share their columns, so S of a tile's next unit waits for its P V; that wait is on the completion of the
-// multiply (multiplies into different accumulators are not ordered by their issue).
+// P is written over its S.  Each group has two such places (one with f32 queries of 128 channels), so the scores of the
+// next 64 keys are made while this step's are turned into weights; a place is taken again once the completion of its P V
+// has been seen (multiplies into different accumulators are not ordered by their issue).  Each group has an issuing warp of its
+// own that waits where it must; one warp polling for both took 1500 cycles a round of its own code.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -32,27 +34,27 @@ namespace {
 
 using namespace tcc;
 
-constexpr int THREADS = 384;             // two groups of 128 rows, the multiply's warp, the copies' warp, the queries' two
-constexpr int SNAP = 2;                  // stretches of up to this many units are not cut
+constexpr int THREADS = 384;             // two groups of 128 rows, a warp per group that issues multiplies, the copies' warp, the queries'
+constexpr int KT = 64;                   // keys per unit
+constexpr int SNAP = 4;                  // stretches of up to this many units are not cut
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by before the sums are rescaled
 
 template <int HS_, int L_>
 struct Shape {
     static constexpr int HS = HS_, L = L_;
-    static constexpr int KT = HS == 128 && L == 3 ? 64 : 128;        // keys per unit
-    static constexpr int QT = HS == 128 && L == 3 ? 1 : 2;           // 128-row tiles per block
+    static constexpr int QT = HS == 128 && L == 3 ? 1 : 2;           // 128-row tiles per block (three limbs of 128 channels: room for one)
     static constexpr int MR = 128 * QT;
     static constexpr int HALVES = HS / 64;                           // 64-channel columns of 128 bytes a row
     static constexpr uint32_t Q_LIMB = 128 * HS * 2, Q_TILE = L * Q_LIMB, KV = KT * HS * 2;
-    static constexpr int NK = HS == 64 ? (L == 1 ? 5 : 3) : (L == 1 ? 3 : 4), NV = HS == 64 ? (L == 1 ? 5 : 3) : (L == 1 ? 2 : 4);
-    static constexpr uint32_t OFF_K = QT * Q_TILE, OFF_V = OFF_K + NK * KV, OFF_BAR = OFF_V + NV * KV, OFF_ML = OFF_BAR + 512;
+    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 8) : (L == 1 ? 5 : 4);   // units of K, and of V, in shared memory
+    static constexpr uint32_t OFF_K = QT * Q_TILE, OFF_V = OFF_K + RING * KV, OFF_BAR = OFF_V + RING * KV, OFF_ML = OFF_BAR + 768;
     static constexpr uint32_t BYTES = OFF_ML + (QT == 1 ? 1024 : 0) + 1024;   // the rest: alignment to 1024
-    // Tensor memory of a group: the scores, the weights' third limbs, the mix.  A stretch of 32 scores is read at once and
-    // its weights go back over it: the first limb in its first 16 columns, the second in its last 16, the third outside.
-    static __device__ __forceinline__ uint32_t weights_at(int l, int c) { return l == 2 ? KT + c / 2 : c + 16 * l; }   // of keys c .. c + 31
-    static constexpr uint32_t C_O = KT == 64 ? 128 : KT + (L == 3 ? KT / 2 : 0), C_GROUP = 256;
-    static_assert(C_O + HS <= C_GROUP, "tensor memory");
+    // Tensor memory of a group: places of scores and weights, the mix.  A place's scores are read 32 columns at a time and
+    // the weights go back over them: the first limb in the first 16 columns, the second in the last 16, the third outside.
+    static __device__ __forceinline__ uint32_t weights_at(int l, int c) { return l == 2 ? 64 + c / 2 : c + 16 * l; }   // of keys c .. c + 31
+    static constexpr uint32_t PLACES = HS == 128 && L == 3 ? 1 : 2, PLACE = L == 3 ? 96 : 64, C_O = HS == 64 && L == 3 ? 192 : 128, GROUP = 256;
+    static_assert(PLACES * PLACE <= C_O && C_O + HS <= GROUP, "tensor memory");
     static_assert(BYTES <= 232448, "shared memory");
 };
 
@@ -135,6 +137,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    tmem_st16(taddr, r);
+    tmem_st16(taddr + 16, r + 16);
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int page, uint64_t* bar) {
@@ -155,10 +161,10 @@ __device__ __forceinline__ uint64_t desc_keys_down(uint32_t at, uint32_t group) 
 }
 
 struct Bars {
-    uint64_t full_k[5], empty_k[5], full_v[5], empty_v[5], q_ready[2], q_free[2], s_ready[2], p_ready[2], pv_done[2], o_free[2];
+    uint64_t full_k[10], empty_k[10], full_v[10], empty_v[10], q_ready[2], q_free[2], s_ready[2][2], p_ready[2][2], pv_done[2][2], o_free[2], passed[10];
     uint32_t tmem, failed;
 };
-static_assert(sizeof(Bars) <= 512, "barriers");
+static_assert(sizeof(Bars) <= 768, "barriers");
 
 // A wait that ends: true when the phase is there, false when it ran out here or anywhere in the block.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
@@ -181,6 +187,16 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile ui
     *failed = 1;
     return false;
 }
+// one lane of a whole warp
+__device__ __forceinline__ bool elected() {
+    uint32_t yes = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "@p mov.u32 %0, 1;\n\t}"
+        : "+r"(yes));
+    return yes != 0;
+}
 // the same answer for the whole warp
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
     return __all_sync(0xffffffffu, wait(bar, parity, failed));
@@ -201,8 +217,8 @@ template <typename Sh>
 __device__ __forceinline__ Run<Sh> run_of(const ReadArgs& a, const split::Item& it, long long u, long long stop) {
     Run<Sh> r;
     const bool none = it.s.lo >= it.s.hi;
-    r.ta = none ? 0 : it.s.lo / Sh::KT + (int)(u - it.begin);
-    r.tb = none ? 0 : it.s.lo / Sh::KT + (int)(stop - it.begin);
+    r.ta = none ? 0 : it.s.lo / KT + (int)(u - it.begin);
+    r.tb = none ? 0 : it.s.lo / KT + (int)(stop - it.begin);
     r.rows = min(it.q.f * a.group - it.tile * Sh::MR, Sh::MR);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -211,8 +227,8 @@ __device__ __forceinline__ Run<Sh> run_of(const ReadArgs& a, const split::Item& 
             const int m0 = it.tile * Sh::MR + 128 * w, m1 = it.tile * Sh::MR + min(r.rows, 128 * w + 128) - 1;
             const int hi = it.q.c + m1 / a.group + 1, lo = a.window > 0 ? max(it.q.first, it.q.c + m0 / a.group + 1 - a.window) : it.q.first;
             if (lo < hi) {
-                r.a[w] = max(r.ta, lo / Sh::KT);
-                r.b[w] = min(r.tb, (hi + Sh::KT - 1) / Sh::KT);
+                r.a[w] = max(r.ta, lo / KT);
+                r.b[w] = min(r.tb, (hi + KT - 1) / KT);
             }
         }
     }
@@ -222,7 +238,8 @@ __device__ __forceinline__ Run<Sh> run_of(const ReadArgs& a, const split::Item& 
 template <typename Sh>
 __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ReadArgs a,
                                                             const int heads_inside, const int box_rows, float* __restrict__ ends, split::Cut* __restrict__ cuts) {
-    constexpr int HS = Sh::HS, L = Sh::L, KT = Sh::KT, QT = Sh::QT, MR = Sh::MR;
+    constexpr int HS = Sh::HS, L = Sh::L, QT = Sh::QT, MR = Sh::MR;
+    constexpr uint32_t RING = Sh::RING, PLACES = Sh::PLACES;
     extern __shared__ unsigned char raw[];
     unsigned char* smem = raw + ((1024u - (s32(raw) & 1023u)) & 1023u);
     const uint32_t at0 = s32(smem);
@@ -236,23 +253,26 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
     if (bad_length && a.status && blockIdx.x == 0) atomicOr(a.status, AVA_PAGED_BAD_LENGTH);
     const int worker = blockIdx.x;
     const long long per = max((line.total() + gridDim.x - 1) / (long long)gridDim.x, 1ll);
-    split::Item it, after;
+    split::Item it = {}, after = {};
     long long u = split::piece<MR, KT, SNAP>(a, line, per, worker, &it);
     const long long end = split::piece<MR, KT, SNAP>(a, line, per, worker + 1ll, &after);
     if (tid == 0) {
         cuts[worker].workers = 0;
-        for (int i = 0; i < 5; ++i) {
+        for (uint32_t i = 0; i < RING; ++i) {
             bar_init(&bars->full_k[i], 1);
-            bar_init(&bars->empty_k[i], 1);
             bar_init(&bars->full_v[i], 1);
-            bar_init(&bars->empty_v[i], 1);
+            bar_init(&bars->empty_k[i], QT);   // every group that the unit could be for has used it or passed it over
+            bar_init(&bars->empty_v[i], QT);
+            bar_init(&bars->passed[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
-            bar_init(&bars->q_ready[w], QT == 2 ? 1 : 2);   // the warps that bring a tile of queries
-            bar_init(&bars->q_free[w], 1);
-            bar_init(&bars->s_ready[w], 1);
-            bar_init(&bars->p_ready[w], 128);
-            bar_init(&bars->pv_done[w], 1);
+            bar_init(&bars->q_ready[w], 1);
+            bar_init(&bars->q_free[w], QT == 2 ? 1 : 2);    // QT 1: both groups have made their last scores from the tile
+            for (uint32_t i = 0; i < PLACES; ++i) {
+                bar_init(&bars->s_ready[w][i], 1);
+                bar_init(&bars->p_ready[w][i], 128);
+                bar_init(&bars->pv_done[w][i], 1);
+            }
             bar_init(&bars->o_free[w], 128);
         }
         bars->failed = 0;
@@ -274,10 +294,10 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
     if (warp < 8) {
         // ---- one row per thread
         const int w = warp >> 2, row = tid & 127, q_row = QT == 2 ? w * 128 + row : row;   // row within the block's tile
-        const uint32_t mine = tmem + w * Sh::C_GROUP + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t mine = tmem + w * Sh::GROUP + ((uint32_t)((warp & 3) * 32) << 16);
         const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;   // its sign is in the queries
         const bool out_wide = !((reinterpret_cast<uintptr_t>(a.out) & 15) || (a.out_token_stride % (L == 3 ? 4 : 8)) || (a.out_head_stride % (L == 3 ? 4 : 8)));
-        uint32_t n_s = 0, n_pv = 0;      // units of this group so far: its barriers' phases
+        uint32_t n_p = 0;                // units of this group so far: its barriers' phases
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
             const bool whole = u == it.begin && stop == it.begin + it.s.units;
@@ -289,19 +309,19 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             float top = -INFINITY, sum = 0.0f;
             for (int n = 0; n < units && ok; ++n) {
                 const int t = QT == 2 ? run.first(w) + n : run.first(w) + 2 * n;
-                ok = warp_wait(&bars->s_ready[w], n_s & 1, failed);
-                ++n_s;
+                const uint32_t place = n_p % PLACES, at = mine + place * Sh::PLACE;
+                ok = warp_wait(&bars->s_ready[w][place], (n_p / PLACES) & 1, failed);
                 if (!ok) break;
                 tc_after();
-                // Both passes over the row go 32 columns at a time, in loops that are not unrolled: straight through, the
-                // code was larger than the instruction caches keep at hand and half the time went into fetching it.
                 const int from = low - t * KT, to = pos - t * KT;   // keys [from, to] of the unit are seen
                 const bool edge = __any_sync(0xffffffffu, from > 0 || to < KT - 1);
                 float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                // Both passes over the row go 32 columns at a time, in loops that are not unrolled: straight through, the code is
+                // larger than the instruction caches keep at hand.
 #pragma unroll 1
                 for (int c = 0; c < KT; c += 32) {
                     uint32_t s[32];
-                    tmem_ld32(mine + c, s);
+                    tmem_ld32(at + c, s);
                     tmem_wait_ld();
                     if (edge) {
 #pragma unroll
@@ -315,7 +335,10 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
                 if (__any_sync(0xffffffffu, grown)) {
                     const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
-                    if (n > 0) {   // the unit before has been added up: its completion is what let these scores be made
+                    if (n > 0) {   // once the unit before has been added up
+                        ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
+                        if (!ok) break;
+                        tc_after();
 #pragma unroll 1
                         for (int c = 0; c < HS; c += 32) {
                             uint32_t o[32];
@@ -323,8 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                             tmem_wait_ld();
 #pragma unroll
                             for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                            tmem_st16(mine + Sh::C_O + c, o);
-                            tmem_st16(mine + Sh::C_O + c + 16, o + 16);
+                            tmem_st32(mine + Sh::C_O + c, o);
                         }
                     }
                     sum *= f;
@@ -336,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
 #pragma unroll 1
                 for (int c = 0; c < KT; c += 32) {
                     uint32_t s[32], p[L][16];
-                    tmem_ld32(mine + c, s);
+                    tmem_ld32(at + c, s);
                     tmem_wait_ld();
                     if (edge) {
 #pragma unroll
@@ -359,18 +381,18 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                         }
                     }
 #pragma unroll
-                    for (int l = 0; l < L; ++l) tmem_st16(mine + Sh::weights_at(l, c), p[l]);
+                    for (int l = 0; l < L; ++l) tmem_st16(at + Sh::weights_at(l, c), p[l]);
                 }
                 float x, y;
                 apart(add2(part[0], part[1]), x, y);
                 sum += x + y;
                 tmem_wait_st();
                 tc_before();
-                bar_arrive(&bars->p_ready[w]);
-                ++n_pv;
+                bar_arrive(&bars->p_ready[w][place]);
+                ++n_p;
             }
             // ---- the read of the row, or this piece's end of it
-            if (units > 0 && ok) ok = warp_wait(&bars->pv_done[w], (n_pv - 1) & 1, failed);
+            if (units > 0 && ok) ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
             if (QT == 2 && !ok) break;
             tc_after();
             float other_f = 0.0f, own_f = 1.0f;
@@ -416,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
 #pragma unroll
                     for (int k = 0; k < 32; ++k) x[k] = units > 0 ? __uint_as_float(o[k]) * own_f : 0.0f;
                     if (QT == 1 && both) {
-                        tmem_ld32(mine + Sh::C_GROUP + Sh::C_O + c, o);
+                        tmem_ld32(mine + Sh::GROUP + Sh::C_O + c, o);
                         tmem_wait_ld();
 #pragma unroll
                         for (int k = 0; k < 32; ++k) x[k] = fmaf(__uint_as_float(o[k]), other_f, x[k]);
@@ -474,95 +496,110 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
         }
-    } else if (warp == 8) {
-        // ---- the multiplies: one thread issues, the warp clears the rows of V that belong to nobody
+    } else if (warp < 10) {
+        // ---- a group's multiplies: one lane issues, the warp clears the rows of V that belong to nobody
         constexpr uint32_t i_s = instr_desc(KT), i_o = instr_desc(HS) | (1u << 16);   // V with its keys down
-        uint32_t tk = 0, tv = 0;                      // units loaded so far: the rings' places and phases
-        uint32_t n_q[2] = {0, 0}, n_o[2] = {0, 0}, n_p[2] = {0, 0};   // tiles of queries, stretches and units of the groups so far
-        const bool one = lane == 0;
+        constexpr int STEP = QT == 1 ? 2 : 1;
+        const int w = warp - 8, tile = QT == 2 ? w : 0;
+        const uint32_t d = tmem + w * Sh::GROUP;
+        uint32_t n_s = 0, n_p = 0, n_run = 0, n_q = 0, base = 0;   // scored, mixed, runs mixed, tiles of queries, units of the rings before this run
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
             const Run<Sh> run = run_of<Sh>(a, it, u, stop);
-            // unit t's scores for the groups that work on it, once what their columns held has been used up
-            auto scores = [&](int w, int t) {
-                const int tile = QT == 2 ? w : 0;
-                if (t == run.first(w) && (QT == 2 || w == 0)) {
-                    ok = ok && warp_wait(&bars->q_ready[tile], n_q[tile] & 1, failed);
-                    ++n_q[tile];
-                }
-                if (n_p[w] > 0) ok = ok && warp_wait(&bars->pv_done[w], (n_p[w] - 1) & 1, failed);
-                const uint32_t slot = tk % Sh::NK;
-                ok = ok && warp_wait(&bars->full_k[slot], (tk / Sh::NK) & 1, failed);
-                if (ok && one) {
-                    tc_after();
-                    const unsigned char* q = smem + tile * Sh::Q_TILE;
-                    const unsigned char* k = smem + Sh::OFF_K + slot * Sh::KV;
+            const int from = QT == 2 ? run.a[w] : run.ta, to = QT == 2 ? run.b[w] : run.tb, start = run.ta + (QT == 1 ? w : 0);
+            int ks = start;                      // the next unit whose keys are to be used
+            bool fresh = run.ta < run.tb && (QT == 1 || from < to);   // the run's queries are still to be waited for
+            auto queries = [&]() {
+                ok = warp_wait(&bars->q_ready[tile], n_q & 1, failed);
+                ++n_q;
+                fresh = false;
+            };
+            auto keys = [&]() {
+                const uint32_t seq = base + (uint32_t)(ks - run.ta), slot = seq % RING;
+                const bool mine = ks >= from && ks < to;
+                if (mine && fresh) queries();
+                ok = ok && warp_wait(&bars->full_k[slot], (seq / RING) & 1, failed);
+                if (mine && n_s >= PLACES) ok = ok && warp_wait(&bars->pv_done[w][n_s % PLACES], ((n_s - PLACES) / PLACES) & 1, failed);
+                if (!ok) return;
+                if (elected()) {
+                    if (mine) {
+                        tc_after();
+                        const unsigned char* q = smem + tile * Sh::Q_TILE;
+                        const unsigned char* k = smem + Sh::OFF_K + slot * Sh::KV;
 #pragma unroll
-                    for (int l = 0; l < L; ++l)
+                        for (int l = 0; l < L; ++l)
 #pragma unroll
-                        for (int c = 0; c < HS / 16; ++c)
-                            mma_ss(tmem + w * Sh::C_GROUP, operand_desc(q + l * Sh::Q_LIMB + (c / 4) * (128 * 128)) + 2u * (c & 3),
-                                   operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l + c > 0);
-                    commit(&bars->s_ready[w]);
-                    if (t == (QT == 2 ? run.b[w] : run.tb) - 1) commit(&bars->q_free[tile]);   // the stretch's last scores of this tile
+                            for (int c = 0; c < HS / 16; ++c)
+                                mma_ss(d + (n_s % PLACES) * Sh::PLACE, operand_desc(q + l * Sh::Q_LIMB + (c / 4) * (128 * 128)) + 2u * (c & 3),
+                                       operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l + c > 0);
+                        commit(&bars->s_ready[w][n_s % PLACES]);
+                        if (ks + STEP >= to) commit(&bars->q_free[tile]);   // the run's last scores of this group
+                        commit(&bars->empty_k[slot]);
+                    } else {
+                        bar_arrive(&bars->empty_k[slot]);
+                    }
                 }
                 __syncwarp();
+                if (mine) ++n_s;
+                ks += STEP;
             };
-            // the unit's keys are free once every group's scores are made (each unit of a run is some group's)
-            auto free_keys = [&]() {
-                if (ok && one) commit(&bars->empty_k[tk % Sh::NK]);
-                ++tk;
-            };
-            if (run.ta < run.tb) {
-                for (int w = 0; w < 2; ++w)
-                    if (run.has(w, run.ta)) scores(w, run.ta);
-                free_keys();
-            }
-            for (int t = run.ta; t < run.tb && ok; ++t) {
-                const uint32_t slot = tv % Sh::NV;
-                ok = warp_wait(&bars->full_v[slot], (tv / Sh::NV) & 1, failed);
+            for (int t = start; t < run.tb && ok; t += STEP) {
+                while (ok && ks < run.tb && ks <= t + STEP * (int)(PLACES - 1)) keys();   // the scores are ahead of the weights by a place
                 if (!ok) break;
-                unsigned char* v = smem + Sh::OFF_V + slot * Sh::KV;
+                const uint32_t seq = base + (uint32_t)(t - run.ta), slot = seq % RING, place = n_p % PLACES;
+                const bool mine = t >= from && t < to, first = t == from + (QT == 1 ? w : 0);
                 const int clear_to = it.s.lo - t * KT, clear_from = it.s.hi - t * KT;   // rows in front of the stretch, and behind it
-                if (clear_to > 0 || clear_from < KT) {
-                    for (int e = lane; e < KT * (HS / 8); e += 32) {
-                        const int key = e / (HS / 8), c = e % (HS / 8);
-                        if (key < clear_to || key >= clear_from) *reinterpret_cast<uint4*>(v + (c / 8) * (KT * 128) + swz128(key, (c & 7) * 8)) = make_uint4(0, 0, 0, 0);
+                ok = warp_wait(&bars->full_v[slot], (seq / RING) & 1, failed);
+                if (ok && mine && (clear_to > 0 || clear_from < KT)) {
+                    unsigned char* v = smem + Sh::OFF_V + slot * Sh::KV;
+                    if (QT == 2 && w == 1 && t >= run.a[0] && t < run.b[0]) {   // the first group clears what both use
+                        ok = warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
+                    } else {
+                        for (int e = lane; e < KT * (HS / 8); e += 32) {
+                            const int key = e / (HS / 8), c = e % (HS / 8);
+                            if (key < clear_to || key >= clear_from) *reinterpret_cast<uint4*>(v + (c / 8) * (KT * 128) + swz128(key, (c & 7) * 8)) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_async();
                     }
-                    fence_async();
                     __syncwarp();
                 }
-                for (int w = 0; w < 2 && ok; ++w) {
-                    if (run.has(w, t)) {
-                        ok = warp_wait(&bars->p_ready[w], n_p[w] & 1, failed);
-                        if (t == run.first(w) && n_o[w] > 0) ok = ok && warp_wait(&bars->o_free[w], (n_o[w] - 1) & 1, failed);
-                        if (!ok) break;
-                        if (one) {
-                            tc_after();
-                            const uint32_t p = tmem + w * Sh::C_GROUP;
-#pragma unroll
-                            for (int l = 0; l < L; ++l)
-#pragma unroll
-                                for (int c = 0; c < KT / 16; ++c)
-                                    mma_ts(p + Sh::C_O, p + Sh::weights_at(l, c / 2 * 32) + 8 * (c & 1), desc_keys_down(s32(v) + c * 2048, KT * 128), i_o,
-                                           t != run.first(w) || l + c > 0);
-                            commit(&bars->pv_done[w]);
-                        }
-                        __syncwarp();
-                        ++n_p[w];
-                        if (t == run.first(w)) ++n_o[w];
-                    }
-                    if (t + 1 < run.tb && run.has(w, t + 1)) scores(w, t + 1);
+                if (QT == 2 && w == 0 && lane == 0) bar_arrive(&bars->passed[slot]);
+                if (mine) {
+                    if (first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);
+                    ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);
                 }
                 if (!ok) break;
-                if (t + 1 < run.tb) free_keys();
-                if (one) commit(&bars->empty_v[slot]);
-                ++tv;
+                if (elected()) {
+                    if (mine) {
+                        tc_after();
+                        const uint32_t at_v = at0 + Sh::OFF_V + slot * Sh::KV;
+#pragma unroll
+                        for (int l = 0; l < L; ++l)
+#pragma unroll
+                            for (int c = 0; c < KT / 16; ++c)
+                                mma_ts(d + Sh::C_O, d + place * Sh::PLACE + Sh::weights_at(l, c / 2 * 32) + 8 * (c & 1), desc_keys_down(at_v + c * 2048, KT * 128), i_o,
+                                       !first || l + c > 0);
+                        commit(&bars->pv_done[w][place]);
+                        commit(&bars->empty_v[slot]);
+                    } else {
+                        bar_arrive(&bars->empty_v[slot]);
+                    }
+                }
+                __syncwarp();
+                if (mine) {
+                    ++n_p;
+                    if (first) ++n_run;
+                }
             }
+            if (QT == 1 && ok && fresh) {        // a run of one unit: the second group gives the queries back all the same
+                queries();
+                if (ok && lane == 0) bar_arrive(&bars->q_free[tile]);
+            }
+            base += (uint32_t)(run.tb - run.ta);
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
         }
-    } else if (warp == 9) {
+    } else if (warp == 10) {
         // ---- the copies: a lane per box
         uint32_t n = 0;
         bool bad_page = false;
@@ -586,7 +623,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 }
 #pragma unroll
                 for (int kv = 0; kv < 2 && ok; ++kv) {
-                    const uint32_t ring = kv ? Sh::NV : Sh::NK, slot = n % ring, turn = n / ring;
+                    const uint32_t slot = n % RING, turn = n / RING;
                     uint64_t* full = kv ? &bars->full_v[slot] : &bars->full_k[slot];
                     uint64_t* empty = kv ? &bars->empty_v[slot] : &bars->empty_k[slot];
                     if (turn > 0) ok = warp_wait(empty, (turn - 1) & 1, failed);
@@ -607,34 +644,36 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         }
         if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
         if (!ok) {   // the copies in flight end before the block does
-            for (uint32_t back = 1; back <= 5; ++back) {
-                if (n >= back && back <= Sh::NK) bar_wait(&bars->full_k[(n - back) % Sh::NK], ((n - back) / Sh::NK) & 1);
-                if (n >= back && back <= Sh::NV) bar_wait(&bars->full_v[(n - back) % Sh::NV], ((n - back) / Sh::NV) & 1);
+            for (uint32_t back = 1; back <= RING && back <= n; ++back) {
+                bar_wait(&bars->full_k[(n - back) % RING], ((n - back) / RING) & 1);
+                bar_wait(&bars->full_v[(n - back) % RING], ((n - back) / RING) & 1);
             }
         }
-    } else if (warp >= 10) {
-        // ---- the queries of the next stretch, while this one's weights are still being made: a warp per tile (QT 1: half of
-        // the tile's rows each) into the operand layout, eight pieces of a row's channels in flight per lane
-        constexpr int CH = L == 3 ? 4 : 8, PIECES = HS / CH, ROWS = QT == 2 ? 128 : 64, AT_ONCE = 8;
-        const int tile = QT == 2 ? warp - 10 : 0, row0 = QT == 2 ? 0 : (warp - 10) * 64;
+    } else {
+        // ---- the queries of the next stretch, while this one's weights are still being made, into the operand layout: eight
+        // pieces of a row's channels in flight per lane
+        constexpr int CH = L == 3 ? 4 : 8, PIECES = HS / CH, AT_ONCE = 8;
         const bool wide = !((reinterpret_cast<uintptr_t>(a.q) & 15) || (a.q_token_stride % CH) || (a.q_head_stride % CH));
         // the scale's sign goes into the queries, so that the largest score is the largest product; a scale of 0 empties them
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
-        unsigned char* to = smem + tile * Sh::Q_TILE;
-        uint32_t n = 0;
+        uint32_t n[2] = {0, 0};
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
             const Run<Sh> run = run_of<Sh>(a, it, u, stop);
-            if (QT == 2 ? run.count(tile) > 0 : run.ta < run.tb) {
-                if (n > 0) ok = warp_wait(&bars->q_free[tile], (n - 1) & 1, failed);
-                if (!ok) break;
-                ++n;
-                for (int e0 = 0; e0 < ROWS * PIECES; e0 += 32 * AT_ONCE) {
+#pragma unroll
+            for (int tile = 0; tile < QT; ++tile) {
+                if (!(QT == 2 ? run.count(tile) > 0 : run.ta < run.tb) || !ok) continue;
+                if (n[tile] > 0) ok = warp_wait(&bars->q_free[tile], (n[tile] - 1) & 1, failed);
+                if (!ok) continue;
+                ++n[tile];
+                unsigned char* to = smem + tile * Sh::Q_TILE;
+#pragma unroll 1
+                for (int e0 = 0; e0 < 128 * PIECES; e0 += 32 * AT_ONCE) {
                     uint4 x[AT_ONCE];
 #pragma unroll
                     for (int k = 0; k < AT_ONCE; ++k) {
                         const int e = e0 + k * 32 + lane, c = (e % PIECES) * CH;
-                        const int m = it.tile * MR + min(tile * 128 + row0 + e / PIECES, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
+                        const int m = it.tile * MR + min(tile * 128 + e / PIECES, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
                         const int64_t from = (int64_t)(it.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride + c;
                         if (wide) {
                             x[k] = *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) + from * (L == 3 ? 4 : 2));
@@ -649,7 +688,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
 #pragma unroll
                     for (int k = 0; k < AT_ONCE; ++k) {
                         const int e = e0 + k * 32 + lane, c = (e % PIECES) * CH;
-                        unsigned char* at = to + (c / 64) * (128 * 128) + swz128(row0 + e / PIECES, c & 63);
+                        unsigned char* at = to + (c / 64) * (128 * 128) + swz128(e / PIECES, c & 63);
                         if constexpr (L == 3) {
                             uint64_t y = two(__uint_as_float(x[k].x), __uint_as_float(x[k].y)), z = two(__uint_as_float(x[k].z), __uint_as_float(x[k].w));
 #pragma unroll
@@ -744,8 +783,8 @@ bool pool_map(CUtensorMap* map, const void* base, const Pool& p, uint32_t box_ro
 template <int HS, int L>
 cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, const Pool& pool, bool* taken) {
     using Sh = Shape<HS, L>;
-    const int box_rows = a.s.page_size < Sh::KT ? a.s.page_size : Sh::KT;
-    if (box_rows < 8 || Sh::KT % box_rows || a.s.page_size % box_rows) return cudaSuccess;
+    const int box_rows = a.s.page_size < KT ? a.s.page_size : KT;
+    if (box_rows < 8 || KT % box_rows || a.s.page_size % box_rows) return cudaSuccess;
     CUtensorMap mk, mv;
     if (!pool_map(&mk, a.s.k, pool, (uint32_t)box_rows) || !pool_map(&mv, a.s.v, pool, (uint32_t)box_rows)) return cudaSuccess;
     *taken = true;
