@@ -34,7 +34,7 @@ namespace {
 
 using namespace tcc;
 
-constexpr int THREADS = 384;             // two groups of 128 rows, a warp per group that issues multiplies, the copies' warp, the queries'
+constexpr int THREADS = 384;             // two groups of 128 rows, a warp per group that issues multiplies, the copies' warp
 constexpr int KT = 64;                   // keys per unit
 constexpr int SNAP = 4;                  // stretches of up to this many units are not cut
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
@@ -161,7 +161,7 @@ __device__ __forceinline__ uint64_t desc_keys_down(uint32_t at, uint32_t group) 
 }
 
 struct Bars {
-    uint64_t full_k[10], empty_k[10], full_v[10], empty_v[10], q_ready[2], q_free[2], s_ready[2][2], p_ready[2][2], pv_done[2][2], o_free[2], passed[10];
+    uint64_t full_k[10], empty_k[10], full_v[10], empty_v[10], q_ready[2], s_ready[2][2], p_ready[2][2], pv_done[2][2], o_free[2], passed[10];
     uint32_t tmem, failed;
 };
 static_assert(sizeof(Bars) <= 768, "barriers");
@@ -197,9 +197,15 @@ __device__ __forceinline__ bool elected() {
         : "+r"(yes));
     return yes != 0;
 }
-// the same answer for the whole warp
+// The same for a whole warp.  (One lane asking for the others, or one lane's branch around waits and multiplies, made the
+// chunk of 16 x 1024 rows 1.4 times slower: multiplies are issued fast only from code that the whole warp runs.)
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
     return __all_sync(0xffffffffu, wait(bar, parity, failed));
+}
+// A warp's arrival: what its lanes have done is done.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(bar);
 }
 
 // A worker's run over one stretch: units [ta, tb) of the store's own KT-key units, and which of them each group works on.
@@ -266,14 +272,13 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             bar_init(&bars->passed[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
-            bar_init(&bars->q_ready[w], 1);
-            bar_init(&bars->q_free[w], QT == 2 ? 1 : 2);    // QT 1: both groups have made their last scores from the tile
+            bar_init(&bars->q_ready[w], 4);   // a group's warps
             for (uint32_t i = 0; i < PLACES; ++i) {
                 bar_init(&bars->s_ready[w][i], 1);
-                bar_init(&bars->p_ready[w][i], 128);
+                bar_init(&bars->p_ready[w][i], 4);
                 bar_init(&bars->pv_done[w][i], 1);
             }
-            bar_init(&bars->o_free[w], 128);
+            bar_init(&bars->o_free[w], 4);
         }
         bars->failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -298,6 +303,64 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;   // its sign is in the queries
         const bool out_wide = !((reinterpret_cast<uintptr_t>(a.out) & 15) || (a.out_token_stride % (L == 3 ? 4 : 8)) || (a.out_head_stride % (L == 3 ? 4 : 8)));
         uint32_t n_p = 0;                // units of this group so far: its barriers' phases
+        // A run's queries, a row per thread, into the operand layout.  They are brought as soon as the scores of the run
+        // before are made, in front of its epilogue, so that the first scores of the next run are ready behind it.
+        constexpr int CH = L == 3 ? 4 : 8;   // channels in 16 bytes
+        const bool q_wide = !((reinterpret_cast<uintptr_t>(a.q) & 15) || (a.q_token_stride % CH) || (a.q_head_stride % CH));
+        // the scale's sign goes into the queries, so that the largest score is the largest product; a scale of 0 empties them
+        const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
+        auto bring = [&](const split::Item& of, const Run<Sh>& run) {
+            const int tile = QT == 2 ? w : 0;
+            if (QT == 2 ? run.count(w) == 0 : run.ta >= run.tb) return;
+            const int m = of.tile * MR + min(q_row, run.rows - 1), i = m / a.group, h = of.head * a.group + (m - i * a.group);
+            const int64_t from = (int64_t)(of.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride;
+            unsigned char* to = smem + tile * Sh::Q_TILE;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HS; c0 += 64) {
+                uint4 x[64 / CH];
+#pragma unroll
+                for (int k = 0; k < 64 / CH; ++k) {
+                    const int64_t at = from + c0 + k * CH;
+                    if (q_wide) {
+                        x[k] = *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) + at * (L == 3 ? 4 : 2));
+                    } else if (L == 3) {
+                        const uint32_t* q = static_cast<const uint32_t*>(a.q) + at;
+                        x[k] = make_uint4(q[0], q[1], q[2], q[3]);
+                    } else {
+                        const uint16_t* q = static_cast<const uint16_t*>(a.q) + at;
+                        x[k] = make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16), q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
+                    }
+                }
+                unsigned char* at = to + (c0 / 64) * (128 * 128);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {   // 8 channels: 16 bytes of a limb
+                    if constexpr (L == 3) {
+                        const uint4 u = x[2 * c], v = x[2 * c + 1];
+                        uint64_t y[4] = {two(__uint_as_float(u.x), __uint_as_float(u.y)), two(__uint_as_float(u.z), __uint_as_float(u.w)),
+                                         two(__uint_as_float(v.x), __uint_as_float(v.y)), two(__uint_as_float(v.z), __uint_as_float(v.w))};
+#pragma unroll
+                        for (int l = 0; l < L; ++l) {
+                            uint32_t p[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) p[k] = (limb(y[k]) ^ sign) & keep;
+                            *reinterpret_cast<uint4*>(at + l * Sh::Q_LIMB + swz128(row, 8 * c)) = make_uint4(p[0], p[1], p[2], p[3]);
+                        }
+                    } else {
+                        const uint4 u = x[c];
+                        *reinterpret_cast<uint4*>(at + swz128(row, 8 * c)) = make_uint4((u.x ^ sign) & keep, (u.y ^ sign) & keep, (u.z ^ sign) & keep, (u.w ^ sign) & keep);
+                    }
+                }
+            }
+            fence_async();
+            warp_arrive(&bars->q_ready[tile]);
+        };
+        auto bring_next = [&](long long stop) {
+            if (stop >= end) return;
+            split::Item then = it;
+            split::next<MR, KT>(a, then);
+            bring(then, run_of<Sh>(a, then, stop, min(end, then.begin + then.s.units)));
+        };
+        if (u < end && (QT == 2 || w == 1)) bring(it, run_of<Sh>(a, it, u, min(end, it.begin + it.s.units)));
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
             const bool whole = u == it.begin && stop == it.begin + it.s.units;
@@ -388,9 +451,10 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 sum += x + y;
                 tmem_wait_st();
                 tc_before();
-                bar_arrive(&bars->p_ready[w][place]);
+                warp_arrive(&bars->p_ready[w][place]);
                 ++n_p;
             }
+            if (QT == 2 && ok) bring_next(stop);   // every score of this run has been made
             // ---- the read of the row, or this piece's end of it
             if (units > 0 && ok) ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
             if (QT == 2 && !ok) break;
@@ -414,6 +478,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     : "memory");
                 ok = off == 0;
                 if (!ok) break;
+                if (w == 1) bring_next(stop);
                 if (w == 0) {
                     const float t1 = ml[row], s1 = ml[128 + row], now = fmaxf(top, t1);
                     own_f = top == -INFINITY ? 0.0f : exp2_fast(top - now);
@@ -492,7 +557,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             }
             tc_before();
             if constexpr (QT == 1) asm volatile("bar.sync 1, 256;" ::: "memory");   // the other group's sums have been read
-            if (units > 0) bar_arrive(&bars->o_free[w]);
+            if (units > 0) warp_arrive(&bars->o_free[w]);
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
         }
@@ -533,7 +598,6 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                                 mma_ss(d + (n_s % PLACES) * Sh::PLACE, operand_desc(q + l * Sh::Q_LIMB + (c / 4) * (128 * 128)) + 2u * (c & 3),
                                        operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l + c > 0);
                         commit(&bars->s_ready[w][n_s % PLACES]);
-                        if (ks + STEP >= to) commit(&bars->q_free[tile]);   // the run's last scores of this group
                         commit(&bars->empty_k[slot]);
                     } else {
                         bar_arrive(&bars->empty_k[slot]);
@@ -549,12 +613,12 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 const uint32_t seq = base + (uint32_t)(t - run.ta), slot = seq % RING, place = n_p % PLACES;
                 const bool mine = t >= from && t < to, first = t == from + (QT == 1 ? w : 0);
                 const int clear_to = it.s.lo - t * KT, clear_from = it.s.hi - t * KT;   // rows in front of the stretch, and behind it
-                ok = warp_wait(&bars->full_v[slot], (seq / RING) & 1, failed);
-                if (ok && mine && (clear_to > 0 || clear_from < KT)) {
+                if (mine && (clear_to > 0 || clear_from < KT)) {
                     unsigned char* v = smem + Sh::OFF_V + slot * Sh::KV;
+                    ok = warp_wait(&bars->full_v[slot], (seq / RING) & 1, failed);
                     if (QT == 2 && w == 1 && t >= run.a[0] && t < run.b[0]) {   // the first group clears what both use
-                        ok = warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
-                    } else {
+                        ok = ok && warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
+                    } else if (ok) {
                         for (int e = lane; e < KT * (HS / 8); e += 32) {
                             const int key = e / (HS / 8), c = e % (HS / 8);
                             if (key < clear_to || key >= clear_from) *reinterpret_cast<uint4*>(v + (c / 8) * (KT * 128) + swz128(key, (c & 7) * 8)) = make_uint4(0, 0, 0, 0);
@@ -564,10 +628,9 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     __syncwarp();
                 }
                 if (QT == 2 && w == 0 && lane == 0) bar_arrive(&bars->passed[slot]);
-                if (mine) {
-                    if (first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);
-                    ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);
-                }
+                ok = ok && warp_wait(&bars->full_v[slot], (seq / RING) & 1, failed);
+                if (mine && first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);
+                if (mine) ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);
                 if (!ok) break;
                 if (elected()) {
                     if (mine) {
@@ -591,10 +654,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     if (first) ++n_run;
                 }
             }
-            if (QT == 1 && ok && fresh) {        // a run of one unit: the second group gives the queries back all the same
-                queries();
-                if (ok && lane == 0) bar_arrive(&bars->q_free[tile]);
-            }
+            if (QT == 1 && ok && fresh) queries();   // a run of one unit: the second group keeps count all the same
             base += (uint32_t)(run.tb - run.ta);
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
@@ -648,65 +708,6 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 bar_wait(&bars->full_k[(n - back) % RING], ((n - back) / RING) & 1);
                 bar_wait(&bars->full_v[(n - back) % RING], ((n - back) / RING) & 1);
             }
-        }
-    } else {
-        // ---- the queries of the next stretch, while this one's weights are still being made, into the operand layout: eight
-        // pieces of a row's channels in flight per lane
-        constexpr int CH = L == 3 ? 4 : 8, PIECES = HS / CH, AT_ONCE = 8;
-        const bool wide = !((reinterpret_cast<uintptr_t>(a.q) & 15) || (a.q_token_stride % CH) || (a.q_head_stride % CH));
-        // the scale's sign goes into the queries, so that the largest score is the largest product; a scale of 0 empties them
-        const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
-        uint32_t n[2] = {0, 0};
-        while (u < end && ok) {
-            const long long stop = min(end, it.begin + it.s.units);
-            const Run<Sh> run = run_of<Sh>(a, it, u, stop);
-#pragma unroll
-            for (int tile = 0; tile < QT; ++tile) {
-                if (!(QT == 2 ? run.count(tile) > 0 : run.ta < run.tb) || !ok) continue;
-                if (n[tile] > 0) ok = warp_wait(&bars->q_free[tile], (n[tile] - 1) & 1, failed);
-                if (!ok) continue;
-                ++n[tile];
-                unsigned char* to = smem + tile * Sh::Q_TILE;
-#pragma unroll 1
-                for (int e0 = 0; e0 < 128 * PIECES; e0 += 32 * AT_ONCE) {
-                    uint4 x[AT_ONCE];
-#pragma unroll
-                    for (int k = 0; k < AT_ONCE; ++k) {
-                        const int e = e0 + k * 32 + lane, c = (e % PIECES) * CH;
-                        const int m = it.tile * MR + min(tile * 128 + e / PIECES, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
-                        const int64_t from = (int64_t)(it.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride + c;
-                        if (wide) {
-                            x[k] = *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) + from * (L == 3 ? 4 : 2));
-                        } else if (L == 3) {
-                            const uint32_t* q = static_cast<const uint32_t*>(a.q) + from;
-                            x[k] = make_uint4(q[0], q[1], q[2], q[3]);
-                        } else {
-                            const uint16_t* q = static_cast<const uint16_t*>(a.q) + from;
-                            x[k] = make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16), q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < AT_ONCE; ++k) {
-                        const int e = e0 + k * 32 + lane, c = (e % PIECES) * CH;
-                        unsigned char* at = to + (c / 64) * (128 * 128) + swz128(e / PIECES, c & 63);
-                        if constexpr (L == 3) {
-                            uint64_t y = two(__uint_as_float(x[k].x), __uint_as_float(x[k].y)), z = two(__uint_as_float(x[k].z), __uint_as_float(x[k].w));
-#pragma unroll
-                            for (int l = 0; l < L; ++l) {
-                                const uint32_t v = limb(y), w = limb(z);
-                                *reinterpret_cast<uint2*>(at + l * Sh::Q_LIMB) = make_uint2((v ^ sign) & keep, (w ^ sign) & keep);
-                            }
-                        } else {
-                            *reinterpret_cast<uint4*>(at) = make_uint4((x[k].x ^ sign) & keep, (x[k].y ^ sign) & keep, (x[k].z ^ sign) & keep, (x[k].w ^ sign) & keep);
-                        }
-                    }
-                }
-                fence_async();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars->q_ready[tile]);
-            }
-            u = stop;
-            if (u < end) split::next<MR, KT>(a, it);
         }
     }
     if (!ok && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_WAIT_RAN_OUT);
