@@ -55,14 +55,18 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// c += a . b over the pairs of limbs whose product is at least 2^-18 of the leading one
+// a . b over the pairs of limbs whose product is at least 2^-18 of the leading one: high += the leading pair, low += the
+// others.  The tensor cores' f32 sums are cut, not rounded, at every addition: one running sum over all limbs and keys
+// lost 4e-6 of a read over 2048 keys, always towards 0.  So the small terms have a sum of their own, and no sum on the
+// tensor cores runs over more than one step's keys.
 template <int LA, int LB>
-__device__ __forceinline__ void mma_limbs(float (&c)[4], const uint32_t (&a)[LA][4], const uint32_t (&b0)[LB], const uint32_t (&b1)[LB]) {
+__device__ __forceinline__ void mma_limbs(float (&high)[4], float (&low)[4], const uint32_t (&a)[LA][4], const uint32_t (&b0)[LB], const uint32_t (&b1)[LB]) {
 #pragma unroll
     for (int i = 0; i < LA; ++i)
 #pragma unroll
         for (int j = 0; j < LB; ++j)
-            if (i + j <= 2) mma16816(c, a[i], b0[j], b1[j]);
+            if (i + j > 0 && i + j <= 2) mma16816(low, a[i], b0[j], b1[j]);
+    mma16816(high, a[0], b0[0], b1[0]);
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -227,13 +231,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
             const uint32_t at_k = ring_at + (uint32_t)(((unsigned)(t - t0) % STAGES) * St::BYTES), at_v = at_k + STEP * St::ROW;
             const unsigned char* st = ring + (at_k - ring_at);
 
-            float s[MT][2][4];
+            float s[MT][2][4], sl[MT][2][4];   // leading products, the others
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[mt][n][i] = 0.0f;
+                    for (int i = 0; i < 4; ++i) s[mt][n][i] = sl[mt][n][i] = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
                 uint32_t b[4][LS];
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) mma_limbs(s[mt][n], qf[mt][kk], b[2 * n], b[2 * n + 1]);
+                    for (int n = 0; n < 2; ++n) mma_limbs(s[mt][n], sl[mt][n], qf[mt][kk], b[2 * n], b[2 * n + 1]);
             }
             // scores in units of log2: hidden keys to -infinity, the running maximum, the weights
             const int j0 = t * STEP;
@@ -266,7 +270,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[mt][n][i] *= scale2;
+                    for (int i = 0; i < 4; ++i) s[mt][n][i] = (L == 3 ? s[mt][n][i] + sl[mt][n][i] : s[mt][n][i]) * scale2;
                 if (edge) {
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
@@ -331,7 +335,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) mma_limbs(acc[mt][2 * n2 + n], wf[mt], b[2 * n], b[2 * n + 1]);
+                    for (int n = 0; n < 2; ++n) {
+                        if constexpr (L == 3) {
+                            float high[4] = {0.0f, 0.0f, 0.0f, 0.0f}, low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_limbs(high, low, wf[mt], b[2 * n], b[2 * n + 1]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[mt][2 * n2 + n][i] += high[i] + low[i];
+                        } else {
+                            mma16816(acc[mt][2 * n2 + n], wf[mt][0], b[2 * n][0], b[2 * n + 1][0]);
+                        }
+                    }
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");

@@ -1,20 +1,20 @@
 // The read of new tokens over a bf16 store in pages when a request brings many rows per key head (prompt chunks, drafted
 // runs with shared key heads): the same o = sum_j softmax_j(scale q . k_j) v_j on tcgen05 tensor cores.
 //
-// A block is a worker of read_split.cuh with tiles of 128 * QT rows and units of KT keys; its piece of the line is walked
+// A block is a worker of read_split.cuh with tiles of 256 rows and units of KT keys; its piece of the line is walked
 // stretch by stretch.  Per unit and 128-row tile: S = Q K^T into tensor memory (Q and K from shared memory), one thread per
 // row turns its row of S into weights with a running maximum and sum, and writes them over S as the bf16 operand of
 // O += P V (P from tensor memory, V from shared memory as it arrived, keys down: the multiply takes it that way).  O stays
 // in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8, so almost never after the first
-// units.  Two groups of 128 threads work on two tiles (QT 2) or on the odd and even units of one (QT 1): while one turns
-// its scores into weights the tensor cores multiply for the other.
+// units.  Two groups of 128 threads work on half a tile each: while one turns its scores into weights the tensor cores
+// multiply for the other.
 // Keys and values come by TMA, a box per page and 64 channels, into rings of their own; a page outside the store, or past
 // the stretch, is a coordinate past the tensor's last page, which TMA fills with zeros without reading.  Rows of V in
 // front of the stretch or behind it (the rest of a page, left padding) are written over with zeros in shared memory before
 // the multiply: a weight of 0 times whatever lies there must be 0.
 // With f32 queries Q and P are three bf16 limbs each (L 3): three products per step instead of one.
 //
-// P is written over its S.  Each group has two such places (one with f32 queries of 128 channels), so the scores of the
+// P is written over its S.  Each group has two such places, so the scores of the
 // next 64 keys are made while this step's are turned into weights; a place is taken again once the completion of its P V
 // has been seen (multiplies into different accumulators are not ordered by their issue).  Each group has an issuing warp of its
 // own that waits where it must; one warp polling for both took 1500 cycles a round of its own code.
@@ -36,6 +36,8 @@ using namespace tcc;
 
 constexpr int THREADS = 384;             // two groups of 128 rows, a warp per group that issues multiplies, the copies' warp
 constexpr int KT = 64;                   // keys per unit
+constexpr int MR = 256;                  // rows of a tile
+constexpr uint32_t PLACES = 2;           // of scores and weights, per group
 constexpr int SNAP = 4;                  // stretches of up to this many units are not cut
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by before the sums are rescaled
@@ -43,18 +45,20 @@ constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by 
 template <int HS_, int L_>
 struct Shape {
     static constexpr int HS = HS_, L = L_;
-    static constexpr int QT = HS == 128 && L == 3 ? 1 : 2;           // 128-row tiles per block (three limbs of 128 channels: room for one)
-    static constexpr int MR = 128 * QT;
     static constexpr int HALVES = HS / 64;                           // 64-channel columns of 128 bytes a row
     static constexpr uint32_t Q_LIMB = 128 * HS * 2, Q_TILE = L * Q_LIMB, KV = KT * HS * 2;
-    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 8) : (L == 1 ? 5 : 4);   // units of K, and of V, in shared memory
-    static constexpr uint32_t OFF_K = QT * Q_TILE, OFF_V = OFF_K + RING * KV, OFF_BAR = OFF_V + RING * KV, OFF_ML = OFF_BAR + 768;
-    static constexpr uint32_t BYTES = OFF_ML + (QT == 1 ? 1024 : 0) + 1024;   // the rest: alignment to 1024
-    // Tensor memory of a group: places of scores and weights, the mix.  A place's scores are read 32 columns at a time and
-    // the weights go back over them: the first limb in the first 16 columns, the second in the last 16, the third outside.
-    static __device__ __forceinline__ uint32_t weights_at(int l, int c) { return l == 2 ? 64 + c / 2 : c + 16 * l; }   // of keys c .. c + 31
-    static constexpr uint32_t PLACES = HS == 128 && L == 3 ? 1 : 2, PLACE = L == 3 ? 96 : 64, C_O = HS == 64 && L == 3 ? 192 : 128, GROUP = 256;
-    static_assert(PLACES * PLACE <= C_O && C_O + HS <= GROUP, "tensor memory");
+    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 8) : 5;   // units of K, and of V, in shared memory
+    static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_V = OFF_K + RING * KV, OFF_BAR = OFF_V + RING * KV;
+    static constexpr uint32_t BYTES = OFF_BAR + 768 + 1024;          // the rest: alignment to 1024
+    // Tensor memory of a group: places of scores and weights, the mix.  A place's scores are read a chunk at a time and the
+    // weights go back over it: the first limb in its first half, the second in the second, the third outside.
+    static __device__ __forceinline__ uint32_t weights_at(int l, int c) { return l == 2 ? 64 + c / 2 : c + CW / 2 * l; }   // of the chunk of keys from c on
+    // Chunks of CW columns.  The tensor cores' f32 sums are cut, not rounded, at every addition (one sum over 2048 keys and
+    // three limbs lost 2e-6 of the read, always towards 0): with f32 queries the mix of every FLUSH units is added up in
+    // registers, and of the limbs the small ones go first.
+    static constexpr int CW = L == 3 ? 16 : 32, FLUSH = L == 3 ? 2 : 0;
+    static constexpr uint32_t PLACE = L == 3 ? 96 : 64, C_O = PLACES * PLACE, GROUP = 256;
+    static_assert(C_O + HS <= GROUP, "tensor memory");   // (three limbs of 128 channels do not fit, nor do their queries: k_pread.cu takes them)
     static_assert(BYTES <= 232448, "shared memory");
 };
 
@@ -85,6 +89,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 // the next limb of a pair: bf16 of it, and what that leaves over
@@ -136,6 +145,29 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[N]) {
+    if constexpr (N == 16) tmem_ld16(taddr, r);
+    else tmem_ld32(taddr, r);
+}
+template <int N>
+__device__ __forceinline__ void tmem_write(uint32_t taddr, const uint32_t (&r)[N]) {
+    if constexpr (N == 8) tmem_st8(taddr, r);
+    else tmem_st16(taddr, r);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
     tmem_st16(taddr, r);
@@ -208,29 +240,23 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     if ((threadIdx.x & 31) == 0) bar_arrive(bar);
 }
 
-// A worker's run over one stretch: units [ta, tb) of the store's own KT-key units, and which of them each group works on.
-template <typename Sh>
+// A worker's run over one stretch: units [ta, tb) of the store's own KT-key units, and of them group w's [a, b).
 struct Run {
     int ta, tb, rows;
-    int a[2], b[2];                      // QT 2: group w works on units [a, b); QT 1: on those of its parity in [ta, tb)
-    __device__ __forceinline__ bool has(int w, int t) const {
-        return Sh::QT == 2 ? t >= a[w] && t < b[w] : t >= ta && t < tb && ((t - ta) & 1) == w;
-    }
-    __device__ __forceinline__ int count(int w) const { return Sh::QT == 2 ? max(b[w] - a[w], 0) : (tb - ta + 1 - w) / 2; }
-    __device__ __forceinline__ int first(int w) const { return Sh::QT == 2 ? a[w] : ta + w; }
+    int a[2], b[2];
+    __device__ __forceinline__ int count(int w) const { return max(b[w] - a[w], 0); }
 };
-template <typename Sh>
-__device__ __forceinline__ Run<Sh> run_of(const ReadArgs& a, const split::Item& it, long long u, long long stop) {
-    Run<Sh> r;
+__device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, long long u, long long stop) {
+    Run r;
     const bool none = it.s.lo >= it.s.hi;
     r.ta = none ? 0 : it.s.lo / KT + (int)(u - it.begin);
     r.tb = none ? 0 : it.s.lo / KT + (int)(stop - it.begin);
-    r.rows = min(it.q.f * a.group - it.tile * Sh::MR, Sh::MR);
+    r.rows = min(it.q.f * a.group - it.tile * MR, MR);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         r.a[w] = r.b[w] = r.ta;
-        if (Sh::QT == 2 && r.rows > 128 * w) {   // the keys that this tile's own rows see
-            const int m0 = it.tile * Sh::MR + 128 * w, m1 = it.tile * Sh::MR + min(r.rows, 128 * w + 128) - 1;
+        if (r.rows > 128 * w) {   // the keys that this group's rows see
+            const int m0 = it.tile * MR + 128 * w, m1 = it.tile * MR + min(r.rows, 128 * w + 128) - 1;
             const int hi = it.q.c + m1 / a.group + 1, lo = a.window > 0 ? max(it.q.first, it.q.c + m0 / a.group + 1 - a.window) : it.q.first;
             if (lo < hi) {
                 r.a[w] = max(r.ta, lo / KT);
@@ -244,8 +270,9 @@ __device__ __forceinline__ Run<Sh> run_of(const ReadArgs& a, const split::Item& 
 template <typename Sh>
 __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ReadArgs a,
                                                             const int heads_inside, const int box_rows, float* __restrict__ ends, split::Cut* __restrict__ cuts) {
-    constexpr int HS = Sh::HS, L = Sh::L, QT = Sh::QT, MR = Sh::MR;
-    constexpr uint32_t RING = Sh::RING, PLACES = Sh::PLACES;
+    constexpr int HS = Sh::HS, L = Sh::L;
+    constexpr uint32_t RING = Sh::RING;
+    constexpr int CW = Sh::CW, FLUSH = Sh::FLUSH;
     extern __shared__ unsigned char raw[];
     unsigned char* smem = raw + ((1024u - (s32(raw) & 1023u)) & 1023u);
     const uint32_t at0 = s32(smem);
@@ -267,8 +294,8 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         for (uint32_t i = 0; i < RING; ++i) {
             bar_init(&bars->full_k[i], 1);
             bar_init(&bars->full_v[i], 1);
-            bar_init(&bars->empty_k[i], QT);   // every group that the unit could be for has used it or passed it over
-            bar_init(&bars->empty_v[i], QT);
+            bar_init(&bars->empty_k[i], 2);   // each group has used it or passed it over
+            bar_init(&bars->empty_v[i], 2);
             bar_init(&bars->passed[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
@@ -298,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
 
     if (warp < 8) {
         // ---- one row per thread
-        const int w = warp >> 2, row = tid & 127, q_row = QT == 2 ? w * 128 + row : row;   // row within the block's tile
+        const int w = warp >> 2, row = tid & 127, q_row = w * 128 + row;   // row within the block's tile
         const uint32_t mine = tmem + w * Sh::GROUP + ((uint32_t)((warp & 3) * 32) << 16);
         const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;   // its sign is in the queries
         const bool out_wide = !((reinterpret_cast<uintptr_t>(a.out) & 15) || (a.out_token_stride % (L == 3 ? 4 : 8)) || (a.out_head_stride % (L == 3 ? 4 : 8)));
@@ -309,12 +336,11 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         const bool q_wide = !((reinterpret_cast<uintptr_t>(a.q) & 15) || (a.q_token_stride % CH) || (a.q_head_stride % CH));
         // the scale's sign goes into the queries, so that the largest score is the largest product; a scale of 0 empties them
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
-        auto bring = [&](const split::Item& of, const Run<Sh>& run) {
-            const int tile = QT == 2 ? w : 0;
-            if (QT == 2 ? run.count(w) == 0 : run.ta >= run.tb) return;
+        auto bring = [&](const split::Item& of, const Run& run) {
+            if (run.count(w) == 0) return;
             const int m = of.tile * MR + min(q_row, run.rows - 1), i = m / a.group, h = of.head * a.group + (m - i * a.group);
             const int64_t from = (int64_t)(of.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride;
-            unsigned char* to = smem + tile * Sh::Q_TILE;
+            unsigned char* to = smem + w * Sh::Q_TILE;
 #pragma unroll 1
             for (int c0 = 0; c0 < HS; c0 += 64) {
                 uint4 x[64 / CH];
@@ -352,26 +378,41 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 }
             }
             fence_async();
-            warp_arrive(&bars->q_ready[tile]);
+            warp_arrive(&bars->q_ready[w]);
         };
         auto bring_next = [&](long long stop) {
             if (stop >= end) return;
             split::Item then = it;
             split::next<MR, KT>(a, then);
-            bring(then, run_of<Sh>(a, then, stop, min(end, then.begin + then.s.units)));
+            bring(then, run_of(a, then, stop, min(end, then.begin + then.s.units)));
         };
-        if (u < end && (QT == 2 || w == 1)) bring(it, run_of<Sh>(a, it, u, min(end, it.begin + it.s.units)));
+        if (u < end) bring(it, run_of(a, it, u, min(end, it.begin + it.s.units)));
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
             const bool whole = u == it.begin && stop == it.begin + it.s.units;
-            const Run<Sh> run = run_of<Sh>(a, it, u, stop);
+            const Run run = run_of(a, it, u, stop);
             const int units = run.count(w);
             const bool live = q_row < run.rows;
             const int m = it.tile * MR + min(q_row, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
             const int pos = it.q.c + i, low = a.window > 0 ? max(it.q.first, pos - a.window + 1) : it.q.first;
             float top = -INFINITY, sum = 0.0f;
+            uint64_t acc[FLUSH ? HS / 2 : 1];    // the mix of the units that have been flushed
+#pragma unroll
+            for (int k = 0; k < (FLUSH ? HS / 2 : 1); ++k) acc[k] = 0ull;
+            auto flush = [&]() {                 // the units before this one have been added up in tensor memory: their sum joins acc
+                ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
+                tc_after();
+#pragma unroll
+                for (int c = 0; c < (FLUSH ? HS : 0); c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(mine + Sh::C_O + c, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) acc[c / 2 + k] = add2(acc[c / 2 + k], two(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])));
+                }
+            };
             for (int n = 0; n < units && ok; ++n) {
-                const int t = QT == 2 ? run.first(w) + n : run.first(w) + 2 * n;
+                const int t = run.a[w] + n;
                 const uint32_t place = n_p % PLACES, at = mine + place * Sh::PLACE;
                 ok = warp_wait(&bars->s_ready[w][place], (n_p / PLACES) & 1, failed);
                 if (!ok) break;
@@ -382,23 +423,28 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 // Both passes over the row go 32 columns at a time, in loops that are not unrolled: straight through, the code is
                 // larger than the instruction caches keep at hand.
 #pragma unroll 1
-                for (int c = 0; c < KT; c += 32) {
-                    uint32_t s[32];
-                    tmem_ld32(at + c, s);
+                for (int c = 0; c < KT; c += CW) {
+                    uint32_t s[CW];
+                    tmem_read(at + c, s);
                     tmem_wait_ld();
                     if (edge) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
+                        for (int j = 0; j < CW; ++j)
                             if (c + j < from || c + j > to) s[j] = 0xff800000u;
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
+                    for (int j = 0; j < CW; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
                 }
                 const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
                 const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
+                bool due = FLUSH && n > 0 && n % (FLUSH ? FLUSH : 1) == 0;
                 if (__any_sync(0xffffffffu, grown)) {
                     const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
-                    if (n > 0) {   // once the unit before has been added up
+                    if (due) {
+                        flush();
+                        if (!ok) break;
+                        due = false;
+                    } else if (n > 0) {   // once the unit before has been added up
                         ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
                         if (!ok) break;
                         tc_after();
@@ -412,6 +458,10 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                             tmem_st32(mine + Sh::C_O + c, o);
                         }
                     }
+                    if constexpr (FLUSH > 0) {
+#pragma unroll
+                        for (int k = 0; k < HS / 2; ++k) acc[k] = mul2(acc[k], two(f, f));
+                    }
                     sum *= f;
                     top = now;
                 }
@@ -419,17 +469,17 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 const uint64_t scales = two(scale2, scale2), bases = two(-base, -base);
                 uint64_t part[2] = {0ull, 0ull};
 #pragma unroll 1
-                for (int c = 0; c < KT; c += 32) {
-                    uint32_t s[32], p[L][16];
-                    tmem_ld32(at + c, s);
+                for (int c = 0; c < KT; c += CW) {
+                    uint32_t s[CW], p[L][CW / 2];
+                    tmem_read(at + c, s);
                     tmem_wait_ld();
                     if (edge) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
+                        for (int j = 0; j < CW; ++j)
                             if (c + j < from || c + j > to) s[j] = 0xff800000u;
                     }
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
+                    for (int k = 0; k < CW / 2; ++k) {
                         float x, y;
                         apart(fma2(two(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scales, bases), x, y);
                         x = exp2_fast(x);
@@ -444,70 +494,48 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                         }
                     }
 #pragma unroll
-                    for (int l = 0; l < L; ++l) tmem_st16(at + Sh::weights_at(l, c), p[l]);
+                    for (int l = 0; l < L; ++l) tmem_write(at + Sh::weights_at(l, c), p[l]);
                 }
                 float x, y;
                 apart(add2(part[0], part[1]), x, y);
                 sum += x + y;
                 tmem_wait_st();
+                if (due) {
+                    flush();
+                    if (!ok) break;
+                }
                 tc_before();
                 warp_arrive(&bars->p_ready[w][place]);
                 ++n_p;
             }
-            if (QT == 2 && ok) bring_next(stop);   // every score of this run has been made
+            if (ok) bring_next(stop);   // every score of this run has been made
             // ---- the read of the row, or this piece's end of it
             if (units > 0 && ok) ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
-            if (QT == 2 && !ok) break;
+            if (!ok) break;
             tc_after();
-            float other_f = 0.0f, own_f = 1.0f;
-            bool both = false;
-            if constexpr (QT == 1) {   // two groups hold parts of one row: the first joins them (their sums lie in the same lanes)
-                float* ml = reinterpret_cast<float*>(smem + Sh::OFF_ML);
-                if (w == 1) {
-                    ml[row] = top;
-                    ml[128 + row] = sum;
-                }
-                uint32_t off;   // one group's failed wait ends both: nobody is left at the barrier
-                asm volatile(
-                    "{\n\t.reg .pred p, q;\n\t"
-                    "setp.ne.u32 p, %1, 0;\n\t"
-                    "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
-                    "selp.u32 %0, 1, 0, q;\n\t}"
-                    : "=r"(off)
-                    : "r"(ok ? 0u : 1u)
-                    : "memory");
-                ok = off == 0;
-                if (!ok) break;
-                if (w == 1) bring_next(stop);
-                if (w == 0) {
-                    const float t1 = ml[row], s1 = ml[128 + row], now = fmaxf(top, t1);
-                    own_f = top == -INFINITY ? 0.0f : exp2_fast(top - now);
-                    other_f = t1 == -INFINITY ? 0.0f : exp2_fast(t1 - now);
-                    sum = sum * own_f + s1 * other_f;
-                    top = now;
-                    both = run.count(1) > 0;
-                }
-            }
-            if (QT == 2 || w == 0) {
+            {
                 const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum) : 1.0f;
                 float* end_of = ends + ((int64_t)worker * 2 + (u == it.begin ? 1 : 0)) * (MR * (HS + 2));
                 const int64_t to = (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride;
-#pragma unroll 1
+#pragma unroll(FLUSH ? HS / 32 : 1)
                 for (int c = 0; c < HS; c += 32) {
                     uint32_t o[32];
                     float x[32];
                     if (units > 0) {
                         tmem_ld32(mine + Sh::C_O + c, o);
                         tmem_wait_ld();
+                        if constexpr (FLUSH > 0) {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                float y, z;
+                                apart(add2(acc[c / 2 + k], two(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1]))), y, z);
+                                o[2 * k] = __float_as_uint(y);
+                                o[2 * k + 1] = __float_as_uint(z);
+                            }
+                        }
                     }
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) x[k] = units > 0 ? __uint_as_float(o[k]) * own_f : 0.0f;
-                    if (QT == 1 && both) {
-                        tmem_ld32(mine + Sh::GROUP + Sh::C_O + c, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) x[k] = fmaf(__uint_as_float(o[k]), other_f, x[k]);
-                    }
+                    for (int k = 0; k < 32; ++k) x[k] = units > 0 ? __uint_as_float(o[k]) : 0.0f;
                     if (!live) continue;
                     if (!whole) {
 #pragma unroll
@@ -556,7 +584,6 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 }
             }
             tc_before();
-            if constexpr (QT == 1) asm volatile("bar.sync 1, 256;" ::: "memory");   // the other group's sums have been read
             if (units > 0) warp_arrive(&bars->o_free[w]);
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
@@ -564,39 +591,35 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
     } else if (warp < 10) {
         // ---- a group's multiplies: one lane issues, the warp clears the rows of V that belong to nobody
         constexpr uint32_t i_s = instr_desc(KT), i_o = instr_desc(HS) | (1u << 16);   // V with its keys down
-        constexpr int STEP = QT == 1 ? 2 : 1;
-        const int w = warp - 8, tile = QT == 2 ? w : 0;
+        const int w = warp - 8;
         const uint32_t d = tmem + w * Sh::GROUP;
         uint32_t n_s = 0, n_p = 0, n_run = 0, n_q = 0, base = 0;   // scored, mixed, runs mixed, tiles of queries, units of the rings before this run
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
-            const Run<Sh> run = run_of<Sh>(a, it, u, stop);
-            const int from = QT == 2 ? run.a[w] : run.ta, to = QT == 2 ? run.b[w] : run.tb, start = run.ta + (QT == 1 ? w : 0);
-            int ks = start;                      // the next unit whose keys are to be used
-            bool fresh = run.ta < run.tb && (QT == 1 || from < to);   // the run's queries are still to be waited for
-            auto queries = [&]() {
-                ok = warp_wait(&bars->q_ready[tile], n_q & 1, failed);
-                ++n_q;
-                fresh = false;
-            };
+            const Run run = run_of(a, it, u, stop);
+            const int from = run.a[w], to = run.b[w];
+            int ks = run.ta;                     // the next unit whose keys are to be used
             auto keys = [&]() {
                 const uint32_t seq = base + (uint32_t)(ks - run.ta), slot = seq % RING;
                 const bool mine = ks >= from && ks < to;
-                if (mine && fresh) queries();
+                if (ks == from && mine) {        // the run's queries
+                    ok = warp_wait(&bars->q_ready[w], n_q & 1, failed);
+                    ++n_q;
+                }
                 ok = ok && warp_wait(&bars->full_k[slot], (seq / RING) & 1, failed);
                 if (mine && n_s >= PLACES) ok = ok && warp_wait(&bars->pv_done[w][n_s % PLACES], ((n_s - PLACES) / PLACES) & 1, failed);
                 if (!ok) return;
                 if (elected()) {
                     if (mine) {
                         tc_after();
-                        const unsigned char* q = smem + tile * Sh::Q_TILE;
+                        const unsigned char* q = smem + w * Sh::Q_TILE;
                         const unsigned char* k = smem + Sh::OFF_K + slot * Sh::KV;
 #pragma unroll
-                        for (int l = 0; l < L; ++l)
+                        for (int l = L - 1; l >= 0; --l)
 #pragma unroll
                             for (int c = 0; c < HS / 16; ++c)
                                 mma_ss(d + (n_s % PLACES) * Sh::PLACE, operand_desc(q + l * Sh::Q_LIMB + (c / 4) * (128 * 128)) + 2u * (c & 3),
-                                       operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l + c > 0);
+                                       operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l < L - 1 || c > 0);
                         commit(&bars->s_ready[w][n_s % PLACES]);
                         commit(&bars->empty_k[slot]);
                     } else {
@@ -605,18 +628,19 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 }
                 __syncwarp();
                 if (mine) ++n_s;
-                ks += STEP;
+                ++ks;
             };
-            for (int t = start; t < run.tb && ok; t += STEP) {
-                while (ok && ks < run.tb && ks <= t + STEP * (int)(PLACES - 1)) keys();   // the scores are ahead of the weights by a place
+            for (int t = run.ta; t < run.tb && ok; ++t) {
+                while (ok && ks < run.tb && ks <= t + (int)(PLACES - 1)) keys();   // the scores are ahead of the weights by a place
                 if (!ok) break;
                 const uint32_t seq = base + (uint32_t)(t - run.ta), slot = seq % RING, place = n_p % PLACES;
-                const bool mine = t >= from && t < to, first = t == from + (QT == 1 ? w : 0);
+                const bool mine = t >= from && t < to, first = t == from;
+                const bool fresh_sum = FLUSH ? (t - from) % (FLUSH ? FLUSH : 1) == 0 : first;
                 const int clear_to = it.s.lo - t * KT, clear_from = it.s.hi - t * KT;   // rows in front of the stretch, and behind it
                 if (mine && (clear_to > 0 || clear_from < KT)) {
                     unsigned char* v = smem + Sh::OFF_V + slot * Sh::KV;
                     ok = warp_wait(&bars->full_v[slot], (seq / RING) & 1, failed);
-                    if (QT == 2 && w == 1 && t >= run.a[0] && t < run.b[0]) {   // the first group clears what both use
+                    if (w == 1 && t >= run.a[0] && t < run.b[0]) {   // the first group clears what both use
                         ok = ok && warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
                     } else if (ok) {
                         for (int e = lane; e < KT * (HS / 8); e += 32) {
@@ -627,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     }
                     __syncwarp();
                 }
-                if (QT == 2 && w == 0 && lane == 0) bar_arrive(&bars->passed[slot]);
+                if (w == 0 && lane == 0) bar_arrive(&bars->passed[slot]);
                 ok = ok && warp_wait(&bars->full_v[slot], (seq / RING) & 1, failed);
                 if (mine && first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);
                 if (mine) ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);
@@ -637,11 +661,11 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                         tc_after();
                         const uint32_t at_v = at0 + Sh::OFF_V + slot * Sh::KV;
 #pragma unroll
-                        for (int l = 0; l < L; ++l)
+                        for (int l = L - 1; l >= 0; --l)
 #pragma unroll
                             for (int c = 0; c < KT / 16; ++c)
-                                mma_ts(d + Sh::C_O, d + place * Sh::PLACE + Sh::weights_at(l, c / 2 * 32) + 8 * (c & 1), desc_keys_down(at_v + c * 2048, KT * 128), i_o,
-                                       !first || l + c > 0);
+                                mma_ts(d + Sh::C_O, d + place * Sh::PLACE + Sh::weights_at(l, 16 * c / CW * CW) + 16 * c % CW / 2, desc_keys_down(at_v + c * 2048, KT * 128), i_o,
+                                       !fresh_sum || l < L - 1 || c > 0);
                         commit(&bars->pv_done[w][place]);
                         commit(&bars->empty_v[slot]);
                     } else {
@@ -654,7 +678,6 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     if (first) ++n_run;
                 }
             }
-            if (QT == 1 && ok && fresh) queries();   // a run of one unit: the second group keeps count all the same
             base += (uint32_t)(run.tb - run.ta);
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
@@ -666,7 +689,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         const int boxes = KT / box_rows * Sh::HALVES;
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
-            const Run<Sh> run = run_of<Sh>(a, it, u, stop);
+            const Run run = run_of(a, it, u, stop);
             const int32_t* pages = a.table + (int64_t)it.r * a.max_pages;
             for (int t = run.ta; t < run.tb && ok; ++t, ++n) {
                 // a box is box_rows keys of one page (a unit's keys may lie within one page or run over several)
@@ -718,7 +741,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
 }
 
 // Joins the ends of the stretches that were cut (see k_pread.cu): a block per worker and eight rows, a warp per row.
-template <int HS, int MR>
+template <int HS>
 __global__ void __launch_bounds__(256) join_rows_kernel(const ReadArgs a, const float* __restrict__ ends, const split::Cut* __restrict__ cuts) {
     pdl_enter();
     const int w = blockIdx.x, n = cuts[w].workers, lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
@@ -793,7 +816,7 @@ cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, 
     float* ends = reinterpret_cast<float*>(cuts + sms);
     cudaError_t rc = launch_serving(read_tc_kernel<Sh>, dim3(sms), dim3(THREADS), Sh::BYTES, st, 1, mk, mv, a, pool.heads_inside ? 1 : 0, box_rows, ends, cuts);
     if (rc != cudaSuccess) return rc;
-    return launch_serving(join_rows_kernel<HS, Sh::MR>, dim3(sms, Sh::MR / 8), dim3(256), 0, st, 1, a, ends, cuts);
+    return launch_serving(join_rows_kernel<HS>, dim3(sms, MR / 8), dim3(256), 0, st, 1, a, ends, cuts);
 }
 
 }  // namespace
@@ -801,9 +824,10 @@ cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, 
 cudaError_t launch_paged_read_tc(cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken) {
     *taken = false;
     Pool pool;
-    if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && a.s.head_size != 128) || (int64_t)a.max_fresh * a.group <= 32 || !nested(a.s, &pool)) return cudaSuccess;
+    if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && !(a.s.head_size == 128 && a.bf16_q)) || (int64_t)a.max_fresh * a.group <= (a.bf16_q ? 32 : 64) || !nested(a.s, &pool))
+        return cudaSuccess;
     if (a.s.head_size == 64) return a.bf16_q ? launch_one<64, 1>(st, a, room, sms, pool, taken) : launch_one<64, 3>(st, a, room, sms, pool, taken);
-    return a.bf16_q ? launch_one<128, 1>(st, a, room, sms, pool, taken) : launch_one<128, 3>(st, a, room, sms, pool, taken);
+    return launch_one<128, 1>(st, a, room, sms, pool, taken);
 }
 
 }  // namespace ava

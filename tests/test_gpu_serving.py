@@ -400,12 +400,13 @@ def test_attend_reads_all_whatever_the_host_believed(T, S, dt, max_fresh):
 
 
 @pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("hs", [64, 128])
 @pytest.mark.parametrize("lengths", [[(30000, 1)], [(9000, 1)] * 3, [(8000, 150), (5, 1)], [(0, 1)] * 1500, [(0, 3000)], [(20, 1)] * 300 + [(20000, 1)]])
-def test_attend_long_and_many(T, S, dt, lengths):
+def test_attend_long_and_many(T, S, dt, lengths, hs):
     rng = np.random.default_rng(len(lengths))
-    x = attend_inputs(T, rng, lengths, 4, 2, 64, 64, dt)
-    out, lse = call_attend(T, S, x, 0.125)
-    check_attend(T, x, out, lse, 0.125)
+    x = attend_inputs(T, rng, lengths, 4, 2, hs, 64, dt)
+    out, lse = call_attend(T, S, x, hs ** -0.5)
+    check_attend(T, x, out, lse, hs ** -0.5)
 
 
 @pytest.mark.parametrize("dt", TYPES)
