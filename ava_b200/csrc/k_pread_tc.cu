@@ -47,7 +47,7 @@ struct Shape {
     static constexpr int HS = HS_, L = L_;
     static constexpr int HALVES = HS / 64;                           // 64-channel columns of 128 bytes a row
     static constexpr uint32_t Q_LIMB = 128 * HS * 2, Q_TILE = L * Q_LIMB, KV = KT * HS * 2;
-    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 8) : 5;   // units of K, and of V, in shared memory
+    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 8) : 5;   // units in shared memory
     static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_V = OFF_K + RING * KV, OFF_BAR = OFF_V + RING * KV;
     static constexpr uint32_t BYTES = OFF_BAR + 768 + 1024;          // the rest: alignment to 1024
     // Tensor memory of a group: places of scores and weights, the mix.  A place's scores are read a chunk at a time and the
@@ -193,7 +193,7 @@ __device__ __forceinline__ uint64_t desc_keys_down(uint32_t at, uint32_t group) 
 }
 
 struct Bars {
-    uint64_t full_k[10], empty_k[10], full_v[10], empty_v[10], q_ready[2], s_ready[2][2], p_ready[2][2], pv_done[2][2], o_free[2], passed[10];
+    uint64_t full[10], empty[10], passed[10], q_ready[2], s_ready[2][2], p_ready[2][2], pv_done[2][2], o_free[2];
     uint32_t tmem, failed;
 };
 static_assert(sizeof(Bars) <= 768, "barriers");
@@ -292,10 +292,8 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
     if (tid == 0) {
         cuts[worker].workers = 0;
         for (uint32_t i = 0; i < RING; ++i) {
-            bar_init(&bars->full_k[i], 1);
-            bar_init(&bars->full_v[i], 1);
-            bar_init(&bars->empty_k[i], 2);   // each group has used it or passed it over
-            bar_init(&bars->empty_v[i], 2);
+            bar_init(&bars->full[i], 1);
+            bar_init(&bars->empty[i], 2);     // each group has used it or passed it over
             bar_init(&bars->passed[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
@@ -593,56 +591,62 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         constexpr uint32_t i_s = instr_desc(KT), i_o = instr_desc(HS) | (1u << 16);   // V with its keys down
         const int w = warp - 8;
         const uint32_t d = tmem + w * Sh::GROUP;
-        uint32_t n_s = 0, n_p = 0, n_run = 0, n_q = 0, base = 0;   // scored, mixed, runs mixed, tiles of queries, units of the rings before this run
+        uint32_t n_s = 0, n_p = 0, n_run = 0, base = 0;   // units scored, mixed; runs; units of the ring before this run
         while (u < end && ok) {
             const long long stop = min(end, it.begin + it.s.units);
             const Run run = run_of(a, it, u, stop);
             const int from = run.a[w], to = run.b[w];
-            int ks = run.ta;                     // the next unit whose keys are to be used
-            auto keys = [&]() {
-                const uint32_t seq = base + (uint32_t)(ks - run.ta), slot = seq % RING;
-                const bool mine = ks >= from && ks < to;
-                if (ks == from && mine) {        // the run's queries
-                    ok = warp_wait(&bars->q_ready[w], n_q & 1, failed);
-                    ++n_q;
+            auto full = [&](int t) {             // unit t has landed
+                const uint32_t seq = base + (uint32_t)(t - run.ta);
+                ok = ok && warp_wait(&bars->full[seq % RING], (seq / RING) & 1, failed);
+            };
+            auto pass = [&](int t) {             // a unit that is the other group's alone
+                full(t);
+                if (ok && lane == 0) {
+                    const uint32_t slot = (base + (uint32_t)(t - run.ta)) % RING;
+                    bar_arrive(&bars->empty[slot]);
+                    if (w == 0) bar_arrive(&bars->passed[slot]);
                 }
-                ok = ok && warp_wait(&bars->full_k[slot], (seq / RING) & 1, failed);
-                if (mine && n_s >= PLACES) ok = ok && warp_wait(&bars->pv_done[w][n_s % PLACES], ((n_s - PLACES) / PLACES) & 1, failed);
+            };
+            auto scores = [&](int t) {           // of unit t, which has landed, into the next place
+                const uint32_t slot = (base + (uint32_t)(t - run.ta)) % RING, place = n_s % PLACES;
                 if (!ok) return;
                 if (elected()) {
-                    if (mine) {
-                        tc_after();
-                        const unsigned char* q = smem + w * Sh::Q_TILE;
-                        const unsigned char* k = smem + Sh::OFF_K + slot * Sh::KV;
+                    tc_after();
+                    const unsigned char* q = smem + w * Sh::Q_TILE;
+                    const unsigned char* k = smem + Sh::OFF_K + slot * Sh::KV;
 #pragma unroll
-                        for (int l = L - 1; l >= 0; --l)
+                    for (int l = L - 1; l >= 0; --l)
 #pragma unroll
-                            for (int c = 0; c < HS / 16; ++c)
-                                mma_ss(d + (n_s % PLACES) * Sh::PLACE, operand_desc(q + l * Sh::Q_LIMB + (c / 4) * (128 * 128)) + 2u * (c & 3),
-                                       operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l < L - 1 || c > 0);
-                        commit(&bars->s_ready[w][n_s % PLACES]);
-                        commit(&bars->empty_k[slot]);
-                    } else {
-                        bar_arrive(&bars->empty_k[slot]);
-                    }
+                        for (int c = 0; c < HS / 16; ++c)
+                            mma_ss(d + place * Sh::PLACE, operand_desc(q + l * Sh::Q_LIMB + (c / 4) * (128 * 128)) + 2u * (c & 3),
+                                   operand_desc(k + (c / 4) * (KT * 128)) + 2u * (c & 3), i_s, l < L - 1 || c > 0);
+                    commit(&bars->s_ready[w][place]);
                 }
                 __syncwarp();
-                if (mine) ++n_s;
-                ++ks;
+                ++n_s;
             };
-            for (int t = run.ta; t < run.tb && ok; ++t) {
-                while (ok && ks < run.tb && ks <= t + (int)(PLACES - 1)) keys();   // the scores are ahead of the weights by a place
-                if (!ok) break;
+            for (int t = run.ta; t < min(from, run.tb) && ok; ++t) pass(t);
+            if (from < to) {
+                ok = ok && warp_wait(&bars->q_ready[w], n_run & 1, failed);
+                // the first two units' scores: what their places held before has been mixed
+#pragma unroll 1
+                for (int t = from; t < min(to, from + (int)PLACES) && ok; ++t) {
+                    full(t);
+                    if (n_s >= PLACES) ok = ok && warp_wait(&bars->pv_done[w][n_s % PLACES], ((n_s - PLACES) / PLACES) & 1, failed);
+                    scores(t);
+                }
+            }
+#pragma unroll 1
+            for (int t = from; t < to && ok; ++t) {
                 const uint32_t seq = base + (uint32_t)(t - run.ta), slot = seq % RING, place = n_p % PLACES;
-                const bool mine = t >= from && t < to, first = t == from;
-                const bool fresh_sum = FLUSH ? (t - from) % (FLUSH ? FLUSH : 1) == 0 : first;
+                const bool first = t == from, fresh_sum = FLUSH ? (t - from) % (FLUSH ? FLUSH : 1) == 0 : first;
                 const int clear_to = it.s.lo - t * KT, clear_from = it.s.hi - t * KT;   // rows in front of the stretch, and behind it
-                if (mine && (clear_to > 0 || clear_from < KT)) {
+                if (clear_to > 0 || clear_from < KT) {
                     unsigned char* v = smem + Sh::OFF_V + slot * Sh::KV;
-                    ok = warp_wait(&bars->full_v[slot], (seq / RING) & 1, failed);
                     if (w == 1 && t >= run.a[0] && t < run.b[0]) {   // the first group clears what both use
-                        ok = ok && warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
-                    } else if (ok) {
+                        ok = warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
+                    } else {
                         for (int e = lane; e < KT * (HS / 8); e += 32) {
                             const int key = e / (HS / 8), c = e % (HS / 8);
                             if (key < clear_to || key >= clear_from) *reinterpret_cast<uint4*>(v + (c / 8) * (KT * 128) + swz128(key, (c & 7) * 8)) = make_uint4(0, 0, 0, 0);
@@ -652,32 +656,31 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     __syncwarp();
                 }
                 if (w == 0 && lane == 0) bar_arrive(&bars->passed[slot]);
-                ok = ok && warp_wait(&bars->full_v[slot], (seq / RING) & 1, failed);
-                if (mine && first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);
-                if (mine) ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);
+                if (t + (int)PLACES < to) full(t + PLACES);          // waited for before the weights are: nothing but the mix and
+                if (first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);   // its completion lies
+                ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);              // between them and the next scores
                 if (!ok) break;
                 if (elected()) {
-                    if (mine) {
-                        tc_after();
-                        const uint32_t at_v = at0 + Sh::OFF_V + slot * Sh::KV;
+                    tc_after();
+                    const uint32_t at_v = at0 + Sh::OFF_V + slot * Sh::KV;
 #pragma unroll
-                        for (int l = L - 1; l >= 0; --l)
+                    for (int l = L - 1; l >= 0; --l)
 #pragma unroll
-                            for (int c = 0; c < KT / 16; ++c)
-                                mma_ts(d + Sh::C_O, d + place * Sh::PLACE + Sh::weights_at(l, 16 * c / CW * CW) + 16 * c % CW / 2, desc_keys_down(at_v + c * 2048, KT * 128), i_o,
-                                       !fresh_sum || l < L - 1 || c > 0);
-                        commit(&bars->pv_done[w][place]);
-                        commit(&bars->empty_v[slot]);
-                    } else {
-                        bar_arrive(&bars->empty_v[slot]);
-                    }
+                        for (int c = 0; c < KT / 16; ++c)
+                            mma_ts(d + Sh::C_O, d + place * Sh::PLACE + Sh::weights_at(l, 16 * c / CW * CW) + 16 * c % CW / 2, desc_keys_down(at_v + c * 2048, KT * 128), i_o,
+                                   !fresh_sum || l < L - 1 || c > 0);
+                    commit(&bars->pv_done[w][place]);
+                    commit(&bars->empty[slot]);
                 }
                 __syncwarp();
-                if (mine) {
-                    ++n_p;
-                    if (first) ++n_run;
+                if (t + (int)PLACES < to) {
+                    ok = warp_wait(&bars->pv_done[w][place], (n_p / PLACES) & 1, failed);
+                    scores(t + PLACES);
                 }
+                ++n_p;
             }
+            for (int t = max(to, run.ta); t < run.tb && ok; ++t) pass(t);
+            if (from < to) ++n_run;
             base += (uint32_t)(run.tb - run.ta);
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
@@ -704,33 +707,25 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                         page = a.s.n_pages;
                     }
                 }
-#pragma unroll
-                for (int kv = 0; kv < 2 && ok; ++kv) {
-                    const uint32_t slot = n % RING, turn = n / RING;
-                    uint64_t* full = kv ? &bars->full_v[slot] : &bars->full_k[slot];
-                    uint64_t* empty = kv ? &bars->empty_v[slot] : &bars->empty_k[slot];
-                    if (turn > 0) ok = warp_wait(empty, (turn - 1) & 1, failed);
-                    if (!ok) break;
-                    if (lane == 0) bar_expect(full, Sh::KV);
-                    __syncwarp();
-                    const uint32_t dst = at0 + (kv ? Sh::OFF_V : Sh::OFF_K) + slot * Sh::KV;
-                    if (lane < boxes) {   // at most 32: boxes of 8 keys and more
-                        const int half = lane / (KT / box_rows);
-                        tma_box(dst + half * (KT * 128) + b * box_rows * 128, kv ? &map_v : &map_k, half * 64, heads_inside ? it.head : place,
-                                heads_inside ? place : it.head, page, full);
-                    }
-                    __syncwarp();
+                const uint32_t slot = n % RING, turn = n / RING;
+                if (turn > 0) ok = warp_wait(&bars->empty[slot], (turn - 1) & 1, failed);
+                if (!ok) break;
+                if (lane == 0) bar_expect(&bars->full[slot], 2 * Sh::KV);
+                __syncwarp();
+                if (lane < boxes) {   // at most 16: boxes of 8 keys and more
+                    const int half = lane / (KT / box_rows), x = heads_inside ? it.head : place, y = heads_inside ? place : it.head;
+                    const uint32_t to = at0 + slot * Sh::KV + half * (KT * 128) + b * box_rows * 128;
+                    tma_box(to + Sh::OFF_K, &map_k, half * 64, x, y, page, &bars->full[slot]);
+                    tma_box(to + Sh::OFF_V, &map_v, half * 64, x, y, page, &bars->full[slot]);
                 }
+                __syncwarp();
             }
             u = stop;
             if (u < end) split::next<MR, KT>(a, it);
         }
         if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
         if (!ok) {   // the copies in flight end before the block does
-            for (uint32_t back = 1; back <= RING && back <= n; ++back) {
-                bar_wait(&bars->full_k[(n - back) % RING], ((n - back) / RING) & 1);
-                bar_wait(&bars->full_v[(n - back) % RING], ((n - back) / RING) & 1);
-            }
+            for (uint32_t back = 1; back <= RING && back <= n; ++back) bar_wait(&bars->full[(n - back) % RING], ((n - back) / RING) & 1);
         }
     }
     if (!ok && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_WAIT_RAN_OUT);
