@@ -25,7 +25,6 @@ namespace ava {
 namespace {
 
 constexpr int STEP = 16;                 // keys per stage
-constexpr int SNAP = 8;                  // stretches of up to this many stages (128 keys) are not cut
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 
 __device__ __forceinline__ uint32_t s32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -92,6 +91,12 @@ struct Stage {
     }
 };
 
+// tiles of MR rows, cut into stages; stretches of up to eight stages (128 keys) are not cut
+template <int MT>
+struct Plan {
+    static constexpr int MR = 16 * MT, KT = STEP, START = 2, SNAP = 8;
+};
+
 // Workspace of one worker's piece: the two ends that may be cut (0: goes on from the worker before, 1: goes on in the
 // next), each MR rows of HS sums, then the rows' maxima (of scores times log2 e) and sums.
 template <int HS, int MR>
@@ -110,15 +115,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
     pdl_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
     bool bad_length = false, bad_page = false;
-    const split::Line line = split::line<MR, STEP>(a, sums, &bad_length);
+    using Pl = Plan<MT>;
+    const split::Line line = split::line<Pl>(a, sums, &bad_length);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (bad_length && a.status && blockIdx.x == 0) atomicOr(a.status, AVA_PAGED_BAD_LENGTH);
 
     const int w = blockIdx.x * WARPS + warp;
     const long long per = max((line.total() + workers - 1) / workers, 1ll);
-    split::Item it, after;
-    long long u = split::piece<MR, STEP, SNAP>(a, line, per, w, &it);
-    const long long end = split::piece<MR, STEP, SNAP>(a, line, per, w + 1ll, &after);
+    split::Item it = {}, after = {};
+    long long u = split::piece<Pl>(a, line, per, w, &it);
+    const long long end = split::piece<Pl>(a, line, per, w + 1ll, &after);
     if (lane == 0) cuts[w].workers = 0;
     unsigned char* ring = smem + warp * STAGES * St::BYTES;
     const uint32_t ring_at = s32(ring);
@@ -129,12 +135,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
     const TS* pool_v = static_cast<const TS*>(a.s.v);
 
     while (u < end) {
-        const long long stop = min(end, it.begin + it.s.units);
-        const bool whole = u == it.begin && stop == it.begin + it.s.units;
+        const split::Share run = split::share<Pl>(it, u, end);
+        const bool whole = run.whole;
         const int rows = min(it.q.f * a.group - it.tile * MR, MR);
         // this warp's keys of the stretch: from step t0 to t1 of the store's own 16-key steps
         const bool none = it.s.lo >= it.s.hi;
-        const int t0 = none ? 0 : it.s.lo / STEP + (int)(u - it.begin), t1 = none ? 0 : it.s.lo / STEP + (int)(stop - it.begin);
+        const int t0 = none ? 0 : it.s.lo / STEP + run.from, t1 = none ? 0 : it.s.lo / STEP + run.to;
         const int32_t* pages = a.table + (int64_t)it.r * a.max_pages;
         const int64_t head_at = (int64_t)it.head * a.s.head_stride;
 
@@ -399,10 +405,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
             cuts[w].r = it.r;
             cuts[w].head = it.head;
             cuts[w].tile = it.tile;
-            cuts[w].workers = (int)((it.begin + it.s.units - 1) / per) - w + 1;
+            cuts[w].workers = (int)split::last_worker<Pl>(it, per) - w + 1;
         }
-        u = stop;
-        if (u < end) split::next<MR, STEP>(a, it);
+        u = run.stop;
+        if (u < end) split::next<Pl>(a, it);
     }
     if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
 }

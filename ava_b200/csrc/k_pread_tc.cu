@@ -35,10 +35,11 @@ namespace {
 using namespace tcc;
 
 constexpr int THREADS = 384;             // two groups of 128 rows, a warp per group that issues multiplies, the copies' warp
-constexpr int KT = 64;                   // keys per unit
-constexpr int MR = 256;                  // rows of a tile
 constexpr uint32_t PLACES = 2;           // of scores and weights, per group
-constexpr int SNAP = 4;                  // stretches of up to this many units are not cut
+struct Plan {                            // of the line: a tile's queries and results take as long as four units
+    static constexpr int MR = 256, KT = 64, START = 4, SNAP = 4;
+};
+constexpr int MR = Plan::MR, KT = Plan::KT;
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by before the sums are rescaled
 
@@ -242,15 +243,20 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 
 // A worker's run over one stretch: units [ta, tb) of the store's own KT-key units, and of them group w's [a, b).
 struct Run {
+    long long stop;
+    bool whole;
     int ta, tb, rows;
     int a[2], b[2];
     __device__ __forceinline__ int count(int w) const { return max(b[w] - a[w], 0); }
 };
-__device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, long long u, long long stop) {
+__device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, long long u, long long end) {
     Run r;
+    const split::Share s = split::share<Plan>(it, u, end);
+    r.stop = s.stop;
+    r.whole = s.whole;
     const bool none = it.s.lo >= it.s.hi;
-    r.ta = none ? 0 : it.s.lo / KT + (int)(u - it.begin);
-    r.tb = none ? 0 : it.s.lo / KT + (int)(stop - it.begin);
+    r.ta = none ? 0 : it.s.lo / KT + s.from;
+    r.tb = none ? 0 : it.s.lo / KT + s.to;
     r.rows = min(it.q.f * a.group - it.tile * MR, MR);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -282,13 +288,13 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
     pdl_enter();
     // this block's piece of the line (the sums lie where the copies will)
     bool bad_length = false;
-    const split::Line line = split::line<MR, KT>(a, reinterpret_cast<long long*>(smem + Sh::OFF_K), &bad_length);
+    const split::Line line = split::line<Plan>(a, reinterpret_cast<long long*>(smem + Sh::OFF_K), &bad_length);
     if (bad_length && a.status && blockIdx.x == 0) atomicOr(a.status, AVA_PAGED_BAD_LENGTH);
     const int worker = blockIdx.x;
     const long long per = max((line.total() + gridDim.x - 1) / (long long)gridDim.x, 1ll);
     split::Item it = {}, after = {};
-    long long u = split::piece<MR, KT, SNAP>(a, line, per, worker, &it);
-    const long long end = split::piece<MR, KT, SNAP>(a, line, per, worker + 1ll, &after);
+    long long u = split::piece<Plan>(a, line, per, worker, &it);
+    const long long end = split::piece<Plan>(a, line, per, worker + 1ll, &after);
     if (tid == 0) {
         cuts[worker].workers = 0;
         for (uint32_t i = 0; i < RING; ++i) {
@@ -381,14 +387,13 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         auto bring_next = [&](long long stop) {
             if (stop >= end) return;
             split::Item then = it;
-            split::next<MR, KT>(a, then);
-            bring(then, run_of(a, then, stop, min(end, then.begin + then.s.units)));
+            split::next<Plan>(a, then);
+            bring(then, run_of(a, then, stop, end));
         };
-        if (u < end) bring(it, run_of(a, it, u, min(end, it.begin + it.s.units)));
+        if (u < end) bring(it, run_of(a, it, u, end));
         while (u < end && ok) {
-            const long long stop = min(end, it.begin + it.s.units);
-            const bool whole = u == it.begin && stop == it.begin + it.s.units;
-            const Run run = run_of(a, it, u, stop);
+            const Run run = run_of(a, it, u, end);
+            const bool whole = run.whole;
             const int units = run.count(w);
             const bool live = q_row < run.rows;
             const int m = it.tile * MR + min(q_row, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
@@ -506,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 warp_arrive(&bars->p_ready[w][place]);
                 ++n_p;
             }
-            if (ok) bring_next(stop);   // every score of this run has been made
+            if (ok) bring_next(run.stop);   // every score of this run has been made
             // ---- the read of the row, or this piece's end of it
             if (units > 0 && ok) ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
             if (!ok) break;
@@ -578,13 +583,13 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     cuts[worker].r = it.r;
                     cuts[worker].head = it.head;
                     cuts[worker].tile = it.tile;
-                    cuts[worker].workers = (int)((it.begin + it.s.units - 1) / per) - worker + 1;
+                    cuts[worker].workers = (int)split::last_worker<Plan>(it, per) - worker + 1;
                 }
             }
             tc_before();
             if (units > 0) warp_arrive(&bars->o_free[w]);
-            u = stop;
-            if (u < end) split::next<MR, KT>(a, it);
+            u = run.stop;
+            if (u < end) split::next<Plan>(a, it);
         }
     } else if (warp < 10) {
         // ---- a group's multiplies: one lane issues, the warp clears the rows of V that belong to nobody
@@ -593,8 +598,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         const uint32_t d = tmem + w * Sh::GROUP;
         uint32_t n_s = 0, n_p = 0, n_run = 0, base = 0;   // units scored, mixed; runs; units of the ring before this run
         while (u < end && ok) {
-            const long long stop = min(end, it.begin + it.s.units);
-            const Run run = run_of(a, it, u, stop);
+            const Run run = run_of(a, it, u, end);
             const int from = run.a[w], to = run.b[w];
             auto full = [&](int t) {             // unit t has landed
                 const uint32_t seq = base + (uint32_t)(t - run.ta);
@@ -682,8 +686,8 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             for (int t = max(to, run.ta); t < run.tb && ok; ++t) pass(t);
             if (from < to) ++n_run;
             base += (uint32_t)(run.tb - run.ta);
-            u = stop;
-            if (u < end) split::next<MR, KT>(a, it);
+            u = run.stop;
+            if (u < end) split::next<Plan>(a, it);
         }
     } else if (warp == 10) {
         // ---- the copies: a lane per box
@@ -691,8 +695,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         bool bad_page = false;
         const int boxes = KT / box_rows * Sh::HALVES;
         while (u < end && ok) {
-            const long long stop = min(end, it.begin + it.s.units);
-            const Run run = run_of(a, it, u, stop);
+            const Run run = run_of(a, it, u, end);
             const int32_t* pages = a.table + (int64_t)it.r * a.max_pages;
             for (int t = run.ta; t < run.tb && ok; ++t, ++n) {
                 // a box is box_rows keys of one page (a unit's keys may lie within one page or run over several)
@@ -720,8 +723,8 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 }
                 __syncwarp();
             }
-            u = stop;
-            if (u < end) split::next<MR, KT>(a, it);
+            u = run.stop;
+            if (u < end) split::next<Plan>(a, it);
         }
         if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
         if (!ok) {   // the copies in flight end before the block does

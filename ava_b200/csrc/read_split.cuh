@@ -5,8 +5,9 @@
 // (request, key head, tile, keys), form one line, and every worker (a warp or a block) takes an equal piece of it, so the
 // shares are even whatever the lengths are: one long sequence, a few long prompts or hundreds of ragged requests.  A
 // worker's piece may begin or end inside a tile's stretch; those two ends go to the workspace as unnormalised sums with
-// their running maximum, and a second kernel joins them (the read itself is then no different from one pass).  Stretches
-// of at most SNAP units are never cut.  The lengths are read on the GPU, so the same launch fits any of them.
+// their running maximum, and a second kernel joins them (the read itself is then no different from one pass).  A tile also
+// costs what lies around its keys (its queries, its results): START units more, in front of the stretch on the line.
+// Stretches of at most SNAP units are never cut.  The lengths are read on the GPU, so the same launch fits any of them.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -43,28 +44,38 @@ struct Stretch {
     int units;
 };
 
-template <int MR, int KT>
+template <typename P>
 __device__ __forceinline__ Stretch stretch(const ReadArgs& a, const Request& q, int tile) {
-    const int m0 = tile * MR, m1 = min(q.f * a.group, m0 + MR) - 1;
+    const int m0 = tile * P::MR, m1 = min(q.f * a.group, m0 + P::MR) - 1;
     const int i0 = m0 / a.group, i1 = m1 / a.group;
     Stretch s;
     s.hi = q.c + i1 + 1;
     s.lo = a.window > 0 ? max(q.first, q.c + i0 + 1 - a.window) : q.first;
-    s.units = s.lo < s.hi ? (s.hi - 1) / KT - s.lo / KT + 1 : 1;   // a tile that sees nothing still has its zeros to write
+    s.units = s.lo < s.hi ? (s.hi - 1) / P::KT - s.lo / P::KT + 1 : 1;   // a tile that sees nothing still has its zeros to write
     return s;
 }
 
-template <int MR>
+template <typename P>
 __device__ __forceinline__ int tiles(const ReadArgs& a, const Request& q) {
-    return (q.f * a.group + MR - 1) / MR;
+    return (q.f * a.group + P::MR - 1) / P::MR;
 }
 
-template <int MR, int KT>
-__device__ __forceinline__ long long request_units(const ReadArgs& a, int r, bool* bad) {
-    const Request q = request(a, r, bad);
+// What one key head of a request takes of the line: by one thread, and by a warp together (a prompt has many tiles).
+template <typename P>
+__device__ __forceinline__ long long head_units(const ReadArgs& a, const Request& q) {
     long long n = 0;
-    for (int t = 0, e = tiles<MR>(a, q); t < e; ++t) n += stretch<MR, KT>(a, q, t).units;
-    return n * a.s.kv_heads;
+    for (int t = 0, e = tiles<P>(a, q); t < e; ++t) n += P::START + stretch<P>(a, q, t).units;
+    return n;
+}
+template <typename P>
+__device__ __forceinline__ long long head_units_warp(const ReadArgs& a, const Request& q) {
+    const int e = tiles<P>(a, q), lane = threadIdx.x & 31;
+    if (e <= 1) return e ? P::START + stretch<P>(a, q, 0).units : 0;
+    long long n = 0;
+    for (int t = lane; t < e; t += 32) n += P::START + stretch<P>(a, q, t).units;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
 }
 
 // Where the line's requests begin: sums[e] units lie before request e * step (e = 0 .. entries), by all threads of a block.
@@ -74,16 +85,23 @@ struct Line {
     __device__ __forceinline__ long long total() const { return sums[entries]; }
 };
 
-template <int MR, int KT>
+template <typename P>
 __device__ __forceinline__ Line line(const ReadArgs& a, long long* sums, bool* bad) {
     Line l;
     l.sums = sums;
     l.step = (a.rows + ENTRIES - 1) / ENTRIES;
     l.entries = (a.rows + l.step - 1) / l.step;
-    for (int e = threadIdx.x; e < l.entries; e += blockDim.x) {
-        long long n = 0;
-        for (int r = e * l.step, end = min(a.rows, r + l.step); r < end; ++r) n += request_units<MR, KT>(a, r, bad);
-        sums[e + 1] = n;
+    if (a.rows < 128) {         // few requests: a warp each, a lane per tile
+        for (int r = threadIdx.x >> 5; r < a.rows; r += blockDim.x >> 5) {
+            const long long n = head_units_warp<P>(a, request(a, r, bad)) * a.s.kv_heads;
+            if ((threadIdx.x & 31) == 0) sums[r + 1] = n;
+        }
+    } else {
+        for (int e = threadIdx.x; e < l.entries; e += blockDim.x) {
+            long long n = 0;
+            for (int r = e * l.step, end = min(a.rows, r + l.step); r < end; ++r) n += head_units<P>(a, request(a, r, bad)) * a.s.kv_heads;
+            sums[e + 1] = n;
+        }
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -112,11 +130,11 @@ struct Item {
     int r, head, tile;
     Request q;
     Stretch s;
-    long long begin;            // the stretch's first unit
+    long long begin;            // where the stretch's START units begin; its own follow
 };
 
-// The stretch that unit u lies in (u < total).
-template <int MR, int KT>
+// The stretch that place u of the line lies in (u < total), by a warp together.
+template <typename P>
 __device__ __forceinline__ Item locate(const ReadArgs& a, const Line& l, long long u) {
     int lo = 0, hi = l.entries;
     while (hi - lo > 1) {       // the last entry whose sum is not above u: empty requests are passed over
@@ -130,27 +148,42 @@ __device__ __forceinline__ Item locate(const ReadArgs& a, const Line& l, long lo
     it.r = lo * l.step;
     long long n = 0;
     for (;; ++it.r) {
-        n = request_units<MR, KT>(a, it.r, &bad);
+        it.q = request(a, it.r, &bad);
+        n = l.step == 1 ? l.sums[lo + 1] - it.begin : head_units_warp<P>(a, it.q) * a.s.kv_heads;
         if (u < it.begin + n) break;
         it.begin += n;
     }
-    it.q = request(a, it.r, &bad);
     n /= a.s.kv_heads;
     it.head = (int)((u - it.begin) / n);
     it.begin += n * it.head;
-    for (it.tile = 0;; ++it.tile) {
-        it.s = stretch<MR, KT>(a, it.q, it.tile);
-        if (u < it.begin + it.s.units) break;
-        it.begin += it.s.units;
+    const int e = tiles<P>(a, it.q), lane = threadIdx.x & 31;
+    for (int t0 = 0;; t0 += 32) {   // 32 tiles at a time
+        const int t = t0 + lane;
+        const int own = t < e ? P::START + stretch<P>(a, it.q, t).units : 0;
+        int inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        const unsigned over = __ballot_sync(0xffffffffu, it.begin + inc > u);
+        if (over) {
+            const int k = __ffs(over) - 1;
+            it.begin += __shfl_sync(0xffffffffu, inc - own, k);
+            it.tile = t0 + k;
+            break;
+        }
+        it.begin += __shfl_sync(0xffffffffu, inc, 31);
     }
+    it.s = stretch<P>(a, it.q, it.tile);
     return it;
 }
 
 // The next stretch of the line (there is one).
-template <int MR, int KT>
+template <typename P>
 __device__ __forceinline__ void next(const ReadArgs& a, Item& it) {
-    it.begin += it.s.units;
-    if (++it.tile == tiles<MR>(a, it.q)) {
+    it.begin += P::START + it.s.units;
+    if (++it.tile == tiles<P>(a, it.q)) {
         it.tile = 0;
         if (++it.head == a.s.kv_heads) {
             it.head = 0;
@@ -159,16 +192,40 @@ __device__ __forceinline__ void next(const ReadArgs& a, Item& it) {
             while (it.q.f == 0);
         }
     }
-    it.s = stretch<MR, KT>(a, it.q, it.tile);
+    it.s = stretch<P>(a, it.q, it.tile);
 }
 
-// The first unit of worker w's piece; one that would fall inside a stretch of at most SNAP units moves to its beginning.
-template <int MR, int KT, int SNAP>
+// Where worker w's piece begins; a place inside a stretch of at most SNAP units, or within START + SNAP / 2 units of a
+// stretch's beginning, moves to that beginning.
+template <typename P>
 __device__ __forceinline__ long long piece(const ReadArgs& a, const Line& l, long long per, long long w, Item* it) {
     const long long u = w * per;
     if (u >= l.total()) return l.total();
-    *it = locate<MR, KT>(a, l, u);
-    return it->s.units <= SNAP ? it->begin : u;
+    *it = locate<P>(a, l, u);
+    return it->s.units <= P::SNAP || u <= it->begin + P::START + P::SNAP / 2 ? it->begin : u;
+}
+
+// A worker's run over one stretch, from place u of the line on: its units [from, to) of the stretch, and where it stops.
+struct Share {
+    int from, to;
+    long long stop;
+    bool whole;
+};
+template <typename P>
+__device__ __forceinline__ Share share(const Item& it, long long u, long long end) {
+    Share s;
+    const long long first = it.begin + P::START;
+    s.stop = min(end, first + it.s.units);
+    s.from = u > first ? (int)(u - first) : 0;
+    s.to = (int)(s.stop - first);
+    s.whole = u == it.begin && s.to == it.s.units;
+    return s;
+}
+// The worker whose piece the stretch's last unit lies in (a stretch that is cut: no beginning of a piece inside it has moved
+// but to its own beginning).
+template <typename P>
+__device__ __forceinline__ long long last_worker(const Item& it, long long per) {
+    return (it.begin + P::START + it.s.units - 1) / per;
 }
 
 // What the joining kernel is told by the worker in whose piece a cut stretch begins.
