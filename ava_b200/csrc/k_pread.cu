@@ -2,23 +2,28 @@
 // store type, page size and layout: o = sum_j softmax_j(scale q . k_j) v_j.
 //
 // One pass with the running maximum and sum per row.  What bounds it is the store's bytes: every key and value is used by
-// a handful of rows only, so the kernel is laid out around keeping loads in flight.  A warp is a worker of its own
-// (read_split.cuh): it walks its piece of the line in steps of 16 keys, its own ring of 16-key stages in shared memory
-// filled by asynchronous 16-byte copies several stages ahead; no barrier joins the warps of a block.  Pages are looked up
-// a key at a time (lane = key), one step before their copies are issued, so any page size and any strides of whole 16
-// bytes go; keys outside the stretch or on a page outside the store are written as zeros and never read.
-// The products run on mma.sync (m16n8k16, bf16 in, f32 sums): 16 rows of queries stand in one operand (a request's tokens
-// and the heads that share the key head), and tcgen05's 128-row tiles would be empty for 7 of 8 rows and more.
+// a handful of rows only, so the kernel is laid out around keeping loads in flight and few instructions around them.  A
+// warp is a worker of its own (read_split.cuh): it walks its piece of the line in steps of 16 keys, its own ring of 16-key
+// stages in shared memory filled several stages ahead; no barrier joins the warps of a block.  Pages of 8 or of a multiple
+// of 16 keys come by TMA, one lane asking for 16 keys at a time (a page outside the store is a coordinate past the tensor's
+// last page: zeros, nothing read); other page sizes and strides that do not nest by asynchronous 16-byte copies, every lane
+// looking up a key.  Values of places that are no key of the stretch are written over with zeros.
+// The products run on mma.sync (m16n8k16, bf16 in, f32 sums) with the keys on the long side: S^T = K Q^T and O^T = V^T P^T,
+// so eight rows of queries (a request's tokens and the heads that share the key head) cost one operand of eight columns;
+// with the queries on the long side a single decoded token paid for 16, and with tcgen05's 128-row tiles it would for 128.
 // f32 queries, f32 stores and the softmax weights of f32 queries are three bf16 limbs each (2^-24 of the value; a store's
 // are made as its elements come out of shared memory), and of two limbed operands' nine products the six down to 2^-18 are
 // taken.  Two limbs (2^-17) were not enough: an error of 2e-6 of the read where f32 sums leave 5e-7.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "ava_math.h"
 #include "bf16_hw.cuh"
 #include "kernels.cuh"
 #include "read_split.cuh"
+#include "paged_map.cuh"
 #include "serving.cuh"
+#include "tc_common.cuh"
 
 namespace ava {
 
@@ -27,7 +32,7 @@ namespace {
 constexpr int STEP = 16;                 // keys per stage
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 
-__device__ __forceinline__ uint32_t s32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+using tcc::s32;
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -80,21 +85,29 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 
-// How a warp lays out its stage: 16 rows of HS elements of K, then of V; the 16-byte pieces of a row are rotated by the
-// row so that eight rows' equal pieces lie in eight bank groups.
+// the transpose of an 8 x 8 tile of bf16 held two to a lane
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// How a warp lays out its stage: K, then V, each in columns of up to 128 bytes a key (what a TMA box with the swizzle of
+// that width leaves): the 16-byte pieces of a column's row are rotated by the row, so that eight rows' equal pieces lie in
+// eight bank groups.
 template <typename TS, int HS>
 struct Stage {
-    static constexpr int ROW = HS * (int)sizeof(TS), PIECES = ROW / 16, BYTES = 2 * STEP * ROW;
+    static constexpr int ROW = HS * (int)sizeof(TS), SEG = ROW < 128 ? ROW : 128, PIECES = ROW / 16, PER_SEG = SEG / 16, POOL = STEP * ROW, BYTES = 2 * POOL;
     static __device__ __forceinline__ uint32_t at(int key, int piece) {
-        const int turn = PIECES >= 8 ? (key & 7) : ((key >> 1) & 3);
-        return (uint32_t)(key * ROW + ((piece ^ turn) << 4));
+        const int turn = PER_SEG >= 8 ? (key & 7) : ((key >> 1) & 3);
+        return (uint32_t)((piece / PER_SEG) * (STEP * SEG) + key * SEG + (((piece % PER_SEG) ^ turn) << 4));
     }
 };
 
 // tiles of MR rows, cut into stages; stretches of up to eight stages (128 keys) are not cut
-template <int MT>
+template <int NQ>
 struct Plan {
-    static constexpr int MR = 16 * MT, KT = STEP, START = 2, SNAP = 8;
+    static constexpr int MR = 8 * NQ, KT = STEP, START = 2, SNAP = 8;
 };
 
 // Workspace of one worker's piece: the two ends that may be cut (0: goes on from the worker before, 1: goes on in the
@@ -104,19 +117,29 @@ struct Ends {
     static constexpr int FLOATS = MR * (HS + 2);
 };
 
-template <typename TS, int L, int HS, int MT, int WARPS, int STAGES>
-__global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, float* __restrict__ ends, split::Cut* __restrict__ cuts, const int workers) {
-    constexpr int MR = 16 * MT, KK = HS / 16, NB = HS / 8;
+// How the keys come (box 0: by copies).
+struct Coming {
+    int box, heads_inside;
+};
+
+template <typename TS, int L, int HS, int NQ, int WARPS, int STAGES>
+__global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ReadArgs a,
+                                                           const Coming coming, float* __restrict__ ends, split::Cut* __restrict__ cuts, const int workers) {
+    constexpr int MR = 8 * NQ, KK = HS / 16, MB = HS / 16;
     constexpr bool F32S = sizeof(TS) == 4;
     constexpr int LS = F32S ? 3 : 1;   // limbs of the store's elements
     using St = Stage<TS, HS>;
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = raw + ((1024u - (s32(raw) & 1023u)) & 1023u);
     __shared__ long long sums[split::ENTRIES + 1];
+    __shared__ uint64_t bars[WARPS * STAGES];
     pdl_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
-    bool bad_length = false, bad_page = false;
-    using Pl = Plan<MT>;
-    const split::Line line = split::line<Pl>(a, sums, &bad_length);
+    bool bad_length = false, bad_page = false, ok = true;
+    if (threadIdx.x < WARPS * STAGES) tcc::bar_init(&bars[threadIdx.x], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    using Pl = Plan<NQ>;
+    const split::Line line = split::line<Pl>(a, sums, &bad_length);   // (joins the block's threads)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (bad_length && a.status && blockIdx.x == 0) atomicOr(a.status, AVA_PAGED_BAD_LENGTH);
 
@@ -127,14 +150,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
     const long long end = split::piece<Pl>(a, line, per, w + 1ll, &after);
     if (lane == 0) cuts[w].workers = 0;
     unsigned char* ring = smem + warp * STAGES * St::BYTES;
+    uint64_t* bar = bars + warp * STAGES;
     const uint32_t ring_at = s32(ring);
+    uint32_t filled = 0;                 // stages asked for by TMA so far (their barriers' phases)
     const float scale2 = a.scale * LOG2E;
-    const bool paired = !((reinterpret_cast<uintptr_t>(a.out) & (a.bf16_q ? 3 : 7)) || (a.out_token_stride & 1) || (a.out_head_stride & 1));
     const int page_shift = (a.s.page_size & (a.s.page_size - 1)) ? -1 : __ffs(a.s.page_size) - 1;
     const TS* pool_k = static_cast<const TS*>(a.s.k);
     const TS* pool_v = static_cast<const TS*>(a.s.v);
 
-    while (u < end) {
+    while (u < end && ok) {
         const split::Share run = split::share<Pl>(it, u, end);
         const bool whole = run.whole;
         const int rows = min(it.q.f * a.group - it.tile * MR, MR);
@@ -143,9 +167,25 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
         const int t0 = none ? 0 : it.s.lo / STEP + run.from, t1 = none ? 0 : it.s.lo / STEP + run.to;
         const int32_t* pages = a.table + (int64_t)it.r * a.max_pages;
         const int64_t head_at = (int64_t)it.head * a.s.head_stride;
+        const uint32_t first_filled = filled;
 
-        // the place of key t * 16 + (lane & 15) in the pools, -1: none
+        // Where a step's keys lie.  By copies: the place of key t * 16 + (lane & 15) in the pools, -1: none.  By TMA: lane b's
+        // box of the step, page * 2^32 + place.
         auto place = [&](int t) -> int64_t {
+            if (coming.box) {
+                const int j = t * STEP + (lane & 1) * coming.box;
+                int page = a.s.n_pages, at = 0;
+                if (t < t1 && (lane & 1) * coming.box < STEP && j < it.s.hi && j + coming.box > it.s.lo) {
+                    const int pi = page_shift >= 0 ? j >> page_shift : j / a.s.page_size;
+                    page = pages[pi];
+                    at = j - pi * a.s.page_size;
+                    if (page < 0 || page >= a.s.n_pages) {
+                        bad_page = true;
+                        page = a.s.n_pages;
+                    }
+                }
+                return ((int64_t)page << 32) | (uint32_t)at;
+            }
             const int j = t * STEP + (lane & 15);
             if (t >= t1 || j < it.s.lo || j >= it.s.hi) return -1;
             const int pi = page_shift >= 0 ? j >> page_shift : j / a.s.page_size;
@@ -157,68 +197,81 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
             return page * a.s.page_stride + (j - pi * a.s.page_size) * a.s.place_stride + head_at;
         };
         auto fetch = [&](int t, int64_t at) {
-            const uint32_t dst = ring_at + (uint32_t)(((unsigned)(t - t0) % STAGES) * St::BYTES);
+            const uint32_t slot = (unsigned)(t - t0) % STAGES, dst = ring_at + slot * St::BYTES;
+            if (coming.box) {
+                uint64_t* full = bar + filled % STAGES;   // (slots and barriers need not be the same ones: both turn in order)
+                if (lane == 0) tcc::bar_expect(full, St::BYTES);
+                __syncwarp();
+                if (lane * coming.box < STEP) {           // one box of 16 keys, or two of 8
+                    const int page = (int)(at >> 32), y = (int)(uint32_t)at;
+#pragma unroll
+                    for (int seg = 0; seg < St::ROW / St::SEG; ++seg) {
+                        const uint32_t to = dst + seg * (STEP * St::SEG) + lane * coming.box * St::SEG;
+                        const int x = seg * (St::SEG / (int)sizeof(TS));
+                        tma_box(to, &map_k, x, coming.heads_inside ? it.head : y, coming.heads_inside ? y : it.head, page, full);
+                        tma_box(to + St::POOL, &map_v, x, coming.heads_inside ? it.head : y, coming.heads_inside ? y : it.head, page, full);
+                    }
+                }
+                ++filled;
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < St::PIECES / 2; ++i) {
                 const int id = i * 32 + lane, key = id / St::PIECES, piece = id % St::PIECES;
                 const int64_t from = __shfl_sync(0xffffffffu, at, key);
                 const int64_t e = (from < 0 ? 0 : from) + piece * (16 / (int)sizeof(TS));
                 copy16(dst + St::at(key, piece), pool_k + e, from >= 0);
-                copy16(dst + STEP * St::ROW + St::at(key, piece), pool_v + e, from >= 0);
+                copy16(dst + St::POOL + St::at(key, piece), pool_v + e, from >= 0);
             }
         };
         __syncwarp();   // the stretch before has been read out of the ring by every lane
-        int64_t coming = -1;
+        int64_t ahead_at = -1;
         if (t0 < t1) {
             int64_t at = place(t0);
 #pragma unroll 1
             for (int s = 0; s < STAGES - 1; ++s) {
-                const int64_t ahead = place(t0 + s + 1);
+                const int64_t next_at = place(t0 + s + 1);
                 if (t0 + s < t1) fetch(t0 + s, at);
                 asm volatile("cp.async.commit_group;" ::: "memory");
-                at = ahead;
+                at = next_at;
             }
-            coming = at;
+            ahead_at = at;
         }
 
-        // queries: row m = tile * MR + 16 mt + g (+ 8), channels 16 kk + 2 tq (+ 8)
-        uint32_t qf[MT][KK][L][4];
-        int pos[MT][2];
+        // queries: column 8 nq + g of the tile (B operand: channels 16 kk + 2 tq (+ 8)); a lane's scores are of columns 2 tq, 2 tq + 1
+        uint32_t qf[NQ][KK][2][L];
+        int pos[NQ][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int m = it.tile * MR + min(16 * mt + g + 8 * half, rows - 1);   // rows beyond the last repeat it: no mask of their own
-                const int i = m / a.group, h = it.head * a.group + (m - i * a.group);
-                pos[mt][half] = it.q.c + i;
-                const int64_t at = (int64_t)(it.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride;
+            for (int half = 0; half < 2; ++half)
+                pos[nq][half] = it.q.c + (it.tile * MR + min(8 * nq + 2 * tq + half, rows - 1)) / a.group;   // columns beyond the last repeat it: no mask of their own
+            const int m = it.tile * MR + min(8 * nq + g, rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
+            const int64_t at = (int64_t)(it.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride;
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
+            for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-                    for (int o = 0; o < 2; ++o) {
-                        const int64_t e = at + 16 * kk + 8 * o + 2 * tq;
-                        if (L == 3) {
-                            const float* q = static_cast<const float*>(a.q) + e;
-                            uint32_t l[L];
-                            limbs(q[0], q[1], l);
-#pragma unroll
-                            for (int x = 0; x < L; ++x) qf[mt][kk][x][2 * o + half] = l[x];
-                        } else {
-                            const uint16_t* q = static_cast<const uint16_t*>(a.q) + e;
-                            qf[mt][kk][0][2 * o + half] = q[0] | ((uint32_t)q[1] << 16);
-                        }
+                for (int o = 0; o < 2; ++o) {
+                    const int64_t e = at + 16 * kk + 8 * o + 2 * tq;
+                    if constexpr (L == 3) {
+                        const float* q = static_cast<const float*>(a.q) + e;
+                        limbs(q[0], q[1], qf[nq][kk][o]);
+                    } else {
+                        const uint16_t* q = static_cast<const uint16_t*>(a.q) + e;
+                        qf[nq][kk][o][0] = q[0] | ((uint32_t)q[1] << 16);
                     }
-            }
+                }
+        }
 
-        float acc[MT][NB][4], top[MT][2], sum[MT][2];
+        float acc[NQ][MB][4], top[NQ][2], sum[NQ][2];   // acc: channels 16 mb + g (+ 8) of columns 2 tq, 2 tq + 1
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            top[mt][0] = top[mt][1] = -INFINITY;
-            sum[mt][0] = sum[mt][1] = 0.0f;
+        for (int nq = 0; nq < NQ; ++nq) {
+            top[nq][0] = top[nq][1] = -INFINITY;
+            sum[nq][0] = sum[nq][1] = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+            for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[mt][n][i] = 0.0f;
+                for (int i = 0; i < 4; ++i) acc[nq][mb][i] = 0.0f;
         }
         // keys that every row of the tile sees need no comparison
         const int all_from = a.window > 0 ? max(it.q.first, it.q.c + (it.tile * MR + rows - 1) / a.group + 1 - a.window) : it.q.first;
@@ -226,177 +279,164 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
 
 #pragma unroll 1
         for (int t = t0; t < t1; ++t) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-            __syncwarp();
+            if (coming.box) {
+                const uint32_t n = first_filled + (unsigned)(t - t0);
+                ok = __all_sync(0xffffffffu, tcc::bar_wait(bar + n % STAGES, (n / STAGES) & 1));
+                if (!ok) break;
+            } else {
+                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+                __syncwarp();
+            }
             {   // the stage read last is free: the step STAGES - 1 ahead goes into it
                 const int ahead = t + STAGES - 1;
-                if (ahead < t1) fetch(ahead, coming);
+                if (ahead < t1) fetch(ahead, ahead_at);
                 asm volatile("cp.async.commit_group;" ::: "memory");
-                coming = place(ahead + 1);
+                ahead_at = place(ahead + 1);
             }
-            const uint32_t at_k = ring_at + (uint32_t)(((unsigned)(t - t0) % STAGES) * St::BYTES), at_v = at_k + STEP * St::ROW;
-            const unsigned char* st = ring + (at_k - ring_at);
+            const uint32_t at_k = ring_at + (uint32_t)(((unsigned)(t - t0) % STAGES) * St::BYTES), at_v = at_k + St::POOL;
+            unsigned char* st = ring + (at_k - ring_at);
+            const int j0 = t * STEP;
+            if (coming.box && (j0 < it.s.lo || j0 + STEP > it.s.hi)) {   // rows of V that are no key of the stretch
+                for (int e = lane; e < STEP * St::PIECES; e += 32) {
+                    const int key = e / St::PIECES;
+                    if (j0 + key < it.s.lo || j0 + key >= it.s.hi) *reinterpret_cast<uint4*>(st + St::POOL + St::at(key, e % St::PIECES)) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next copy into this stage comes after
+                __syncwarp();
+            }
 
-            float s[MT][2][4], sl[MT][2][4];   // leading products, the others
+            float s[NQ][4], sl[NQ][4];   // leading products, the others: keys g, g + 8 of columns 2 tq, 2 tq + 1
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[mt][n][i] = sl[mt][n][i] = 0.0f;
+                for (int i = 0; i < 4; ++i) s[nq][i] = sl[nq][i] = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                uint32_t b[4][LS];
+                uint32_t kf[LS][4];      // keys x channels: (g, 2 tq), (g + 8, 2 tq), (g, 2 tq + 8), (g + 8, 2 tq + 8)
                 if constexpr (F32S) {
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int i = 0; i < 4; ++i) {
+                        const int ch = 16 * kk + 8 * (i >> 1) + 2 * tq;
+                        const float2 x = *reinterpret_cast<const float2*>(st + St::at(g + 8 * (i & 1), ch / 4) + (ch & 3) * 4);
+                        uint32_t l[LS];
+                        limbs(x.x, x.y, l);
 #pragma unroll
-                        for (int o = 0; o < 2; ++o) {
-                            const int ch = 16 * kk + 8 * o + 2 * tq;
-                            const float2 x = *reinterpret_cast<const float2*>(st + St::at(8 * n + g, ch / 4) + (ch & 3) * 4);
-                            limbs(x.x, x.y, b[2 * n + o]);
-                        }
+                        for (int y = 0; y < LS; ++y) kf[y][i] = l[y];
+                    }
                 } else {
-                    uint32_t x[4];
-                    ldmatrix4(at_k + St::at((lane & 7) + 8 * (lane >> 4), 2 * kk + ((lane >> 3) & 1)), x);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) b[i][0] = x[i];
+                    ldmatrix4(at_k + St::at((lane & 7) + 8 * ((lane >> 3) & 1), 2 * kk + (lane >> 4)), kf[0]);
                 }
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) mma_limbs(s[mt][n], sl[mt][n], qf[mt][kk], b[2 * n], b[2 * n + 1]);
+                for (int nq = 0; nq < NQ; ++nq) mma_limbs(s[nq], sl[nq], kf, qf[nq][kk][0], qf[nq][kk][1]);
             }
             // scores in units of log2: hidden keys to -infinity, the running maximum, the weights
-            const int j0 = t * STEP;
             const bool edge = j0 < all_from || j0 + STEP > all_to;
-            uint32_t wf[MT][L][4];
+            uint32_t wf[NQ][2][L];       // weights as the other operand: keys 2 tq, 2 tq + 1 (+ 8) of column g
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[mt][n][i] = (L == 3 ? s[mt][n][i] + sl[mt][n][i] : s[mt][n][i]) * scale2;
+                for (int i = 0; i < 4; ++i) s[nq][i] = (L == 3 ? s[nq][i] + sl[nq][i] : s[nq][i]) * scale2;
                 if (edge) {
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int j = j0 + 8 * n + 2 * tq + (i & 1), p = pos[mt][i >> 1];
-                            if (j > p || j < it.q.first || (a.window > 0 && j <= p - a.window)) s[mt][n][i] = -INFINITY;
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = j0 + g + 8 * (i >> 1), p = pos[nq][i & 1];
+                        if (j > p || j < it.q.first || (a.window > 0 && j <= p - a.window)) s[nq][i] = -INFINITY;
+                    }
                 }
-                float high[2];
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-                    high[half] = fmaxf(fmaxf(s[mt][0][2 * half], s[mt][0][2 * half + 1]), fmaxf(s[mt][1][2 * half], s[mt][1][2 * half + 1]));
-                if (__any_sync(0xffffffffu, high[0] > top[mt][0] || high[1] > top[mt][1])) {
+                const float high[2] = {fmaxf(s[nq][0], s[nq][2]), fmaxf(s[nq][1], s[nq][3])};
+                if (__any_sync(0xffffffffu, high[0] > top[nq][0] || high[1] > top[nq][1])) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        float x = fmaxf(high[half], __shfl_xor_sync(0xffffffffu, high[half], 1));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                        x = fmaxf(x, top[mt][half]);
-                        const float f = top[mt][half] == -INFINITY ? 0.0f : exp2_fast(top[mt][half] - x);
-                        top[mt][half] = x;
-                        sum[mt][half] *= f;
+                        float x = high[half];
 #pragma unroll
-                        for (int n = 0; n < NB; ++n) {
-                            acc[mt][n][2 * half] *= f;
-                            acc[mt][n][2 * half + 1] *= f;
+                        for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                        x = fmaxf(x, top[nq][half]);
+                        const float f = top[nq][half] == -INFINITY ? 0.0f : exp2_fast(top[nq][half] - x);
+                        top[nq][half] = x;
+                        sum[nq][half] *= f;
+#pragma unroll
+                        for (int mb = 0; mb < MB; ++mb) {
+                            acc[nq][mb][half] *= f;
+                            acc[nq][mb][2 + half] *= f;
                         }
                     }
                 }
+                const float base[2] = {top[nq][0] == -INFINITY ? 0.0f : top[nq][0], top[nq][1] == -INFINITY ? 0.0f : top[nq][1]};
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const float base = top[mt][half] == -INFINITY ? 0.0f : top[mt][half];
+                for (int o = 0; o < 2; ++o) {
+                    const float x = exp2_fast(s[nq][2 * o] - base[0]), y = exp2_fast(s[nq][2 * o + 1] - base[1]);
+                    sum[nq][0] += x;
+                    sum[nq][1] += y;
+                    uint32_t l[L];
+                    limbs(x, y, l);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const float x = exp2_fast(s[mt][n][2 * half] - base), y = exp2_fast(s[mt][n][2 * half + 1] - base);
-                        sum[mt][half] += x + y;
-                        uint32_t l[L];
-                        limbs(x, y, l);
-#pragma unroll
-                        for (int i = 0; i < L; ++i) wf[mt][i][2 * n + half] = l[i];
-                    }
+                    for (int i = 0; i < L; ++i) wf[nq][o][i] = transposed(l[i]);
                 }
             }
 #pragma unroll
-            for (int n2 = 0; n2 < NB / 2; ++n2) {
-                uint32_t b[4][LS];
+            for (int mb = 0; mb < MB; ++mb) {
+                uint32_t vf[LS][4];      // channels x keys: (g, 2 tq), (g + 8, 2 tq), (g, 2 tq + 8), (g + 8, 2 tq + 8)
                 if constexpr (F32S) {
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int i = 0; i < 4; ++i) {
+                        const int ch = 16 * mb + 8 * (i & 1) + g, key = 8 * (i >> 1) + 2 * tq;
+                        const unsigned char* v = st + St::POOL + (ch & 3) * 4;
+                        uint32_t l[LS];
+                        limbs(*reinterpret_cast<const float*>(v + St::at(key, ch / 4)), *reinterpret_cast<const float*>(v + St::at(key + 1, ch / 4)), l);
 #pragma unroll
-                        for (int o = 0; o < 2; ++o) {
-                            const int ch = 16 * n2 + 8 * n + g, key = 8 * o + 2 * tq;
-                            const unsigned char* v = st + STEP * St::ROW + (ch & 3) * 4;
-                            limbs(*reinterpret_cast<const float*>(v + St::at(key, ch / 4)), *reinterpret_cast<const float*>(v + St::at(key + 1, ch / 4)), b[2 * n + o]);
-                        }
+                        for (int y = 0; y < LS; ++y) vf[y][i] = l[y];
+                    }
                 } else {
-                    uint32_t x[4];
-                    ldmatrix4_trans(at_v + St::at((lane & 7) + 8 * ((lane >> 3) & 1), 2 * n2 + (lane >> 4)), x);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) b[i][0] = x[i];
+                    ldmatrix4_trans(at_v + St::at((lane & 7) + 8 * (lane >> 4), 2 * mb + ((lane >> 3) & 1)), vf[0]);
                 }
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int nq = 0; nq < NQ; ++nq) {
+                    if constexpr (L == 3) {
+                        float high[4] = {0.0f, 0.0f, 0.0f, 0.0f}, low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_limbs(high, low, vf, wf[nq][0], wf[nq][1]);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        if constexpr (L == 3) {
-                            float high[4] = {0.0f, 0.0f, 0.0f, 0.0f}, low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_limbs(high, low, wf[mt], b[2 * n], b[2 * n + 1]);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[mt][2 * n2 + n][i] += high[i] + low[i];
-                        } else {
-                            mma16816(acc[mt][2 * n2 + n], wf[mt][0], b[2 * n][0], b[2 * n + 1][0]);
-                        }
+                        for (int i = 0; i < 4; ++i) acc[nq][mb][i] += high[i] + low[i];
+                    } else {
+                        mma16816(acc[nq][mb], vf[0], wf[nq][0][0], wf[nq][1][0]);
                     }
+                }
             }
+            __syncwarp();   // every lane has read the stage: the next copies may go into it
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!ok) break;
 
-        // the rows' sums over the quad, then the read itself or this piece's end of it
+        // the rows' sums over the lanes that share a column, then the read itself or this piece's end of it
         float* part = ends + ((int64_t)w * 2 + (u == it.begin ? 1 : 0)) * Ends<HS, MR>::FLOATS;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                float l = sum[mt][half];
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                const int row = 16 * mt + g + 8 * half;
+                float l = sum[nq][half];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+                const int row = 8 * nq + 2 * tq + half;
                 if (row >= rows) continue;
                 if (whole) {
                     const float inv = l > 0.0f ? 1.0f / l : l;   // a sum that is NaN stays NaN
                     const int m = it.tile * MR + row, i = m / a.group, h = it.head * a.group + (m - i * a.group);
-                    const int64_t to = (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride + 2 * tq;
+                    const int64_t to = (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride + g;
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        const float x = acc[mt][n][2 * half] * inv, y = acc[mt][n][2 * half + 1] * inv;
-                        if (L == 1) {
-                            uint16_t* o = static_cast<uint16_t*>(a.out) + to + 8 * n;
-                            const uint32_t v = pack_bf16(x, y);
-                            if (paired) *reinterpret_cast<uint32_t*>(o) = v;
-                            else {
-                                o[0] = (uint16_t)v;
-                                o[1] = (uint16_t)(v >> 16);
-                            }
-                        } else {
-                            float* o = static_cast<float*>(a.out) + to + 8 * n;
-                            if (paired) *reinterpret_cast<float2*>(o) = make_float2(x, y);
-                            else {
-                                o[0] = x;
-                                o[1] = y;
-                            }
+                    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                        for (int o = 0; o < 2; ++o) {
+                            const float x = acc[nq][mb][2 * o + half] * inv;
+                            if constexpr (L == 1) static_cast<uint16_t*>(a.out)[to + 16 * mb + 8 * o] = bf16_rn_hw(x);
+                            else static_cast<float*>(a.out)[to + 16 * mb + 8 * o] = x;
                         }
-                    }
-                    if (a.lse && tq == 0) a.lse[(int64_t)(it.q.start + i) * a.heads + h] = l == 0.0f ? -INFINITY : (top[mt][half] + log2f(l)) * LN2;
+                    if (a.lse && g == 0) a.lse[(int64_t)(it.q.start + i) * a.heads + h] = l == 0.0f ? -INFINITY : (top[nq][half] + log2f(l)) * LN2;
                 } else {
 #pragma unroll
-                    for (int n = 0; n < NB; ++n)
-                        *reinterpret_cast<float2*>(part + row * HS + 8 * n + 2 * tq) = make_float2(acc[mt][n][2 * half], acc[mt][n][2 * half + 1]);
-                    if (tq == 0) {
-                        part[MR * HS + row] = top[mt][half];
+                    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                        for (int o = 0; o < 2; ++o) part[row * HS + 16 * mb + 8 * o + g] = acc[nq][mb][2 * o + half];
+                    if (g == 0) {
+                        part[MR * HS + row] = top[nq][half];
                         part[MR * HS + MR + row] = l;
                     }
                 }
@@ -410,12 +450,68 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const ReadArgs a, f
         u = run.stop;
         if (u < end) split::next<Pl>(a, it);
     }
+    if (!ok) {   // the copies in flight end before the warp does
+        for (uint32_t back = 1; back <= STAGES && back <= filled; ++back) tcc::bar_wait(bar + (filled - back) % STAGES, ((filled - back) / STAGES) & 1);
+        if (lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_WAIT_RAN_OUT);
+    }
     if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
 }
 
 // Joins the ends of the stretches that were cut: one block per worker, idle unless a cut stretch begins in its piece.
 // With the parts' maxima m_i, sums l_i and mixes o_i: m = max m_i, out = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
-constexpr int JOIN_WARPS = 8;
+// A warp takes a row: the parts' maxima and sums a lane each, then all lanes the parts' mixes, whose loads depend on nothing
+// but the weights.  Stretches of many parts (a long sequence) have the block's warps share a row's parts.
+constexpr int JOIN_WARPS = 8, SHARED_PARTS = 16;
+
+// the parts k = k0, k0 + step, ... < n of a row: their common maximum, sum and mix
+template <int HS, int MR>
+__device__ __forceinline__ void join_parts(const float* ends, int w, int row, int n, int k0, int step, float& m, float& l, float (&o)[HS / 32]) {
+    constexpr int PER = HS / 32;
+    const int lane = threadIdx.x & 31;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = 0.0f;
+    for (int b = k0; b < n; b += 32 * step) {
+        const int mine = b + lane * step;
+        auto part_of = [&](int k) { return ends + ((int64_t)(w + k) * 2 + (k == 0 ? 1 : 0)) * Ends<HS, MR>::FLOATS; };
+        const float mk = mine < n ? part_of(mine)[MR * HS + row] : -INFINITY, lk = mine < n ? part_of(mine)[MR * HS + MR + row] : 0.0f;
+        float now = mk;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, x));
+        now = fmaxf(now, m);
+        const float before = m == -INFINITY ? 0.0f : exp2_fast(m - now), weight = mk == -INFINITY ? 0.0f : exp2_fast(mk - now);
+        float s = lk * weight;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        l = l * before + s;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) o[i] *= before;
+        const int count = min(32, (n - b + step - 1) / step);
+#pragma unroll 4
+        for (int k = 0; k < count; ++k) {
+            const float wk = __shfl_sync(0xffffffffu, weight, k);
+            const float* part = part_of(b + k * step) + row * HS + lane;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) o[i] = fmaf(part[32 * i], wk, o[i]);
+        }
+        m = now;
+    }
+}
+template <int HS>
+__device__ __forceinline__ void join_write(const ReadArgs& a, const split::Request& q, int head, int m_row, float m, float l, const float (&o)[HS / 32]) {
+    const int lane = threadIdx.x & 31;
+    const float inv = l > 0.0f ? 1.0f / l : l;
+    const int i = m_row / a.group, h = head * a.group + (m_row - i * a.group);
+    const int64_t to = (int64_t)(q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride + lane;
+#pragma unroll
+    for (int c = 0; c < HS / 32; ++c) {
+        if (a.bf16_q) static_cast<uint16_t*>(a.out)[to + 32 * c] = bf16_rn_hw(o[c] * inv);
+        else static_cast<float*>(a.out)[to + 32 * c] = o[c] * inv;
+    }
+    if (a.lse && lane == 0) a.lse[(int64_t)(q.start + i) * a.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
 template <int HS, int MR>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const ReadArgs a, const float* __restrict__ ends, const split::Cut* __restrict__ cuts) {
     pdl_enter();
@@ -427,19 +523,16 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const ReadArgs a,
     bool bad = false;
     const split::Request q = split::request(a, cuts[w].r, &bad);
     const int head = cuts[w].head, tile = cuts[w].tile, rows = min(q.f * a.group - tile * MR, MR);
-    for (int row = 0; row < rows; ++row) {
-        float m = -INFINITY, l = 0.0f, o[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) o[i] = 0.0f;
-        for (int k = warp; k < n; k += JOIN_WARPS) {
-            const float* part = ends + ((int64_t)(w + k) * 2 + (k == 0 ? 1 : 0)) * Ends<HS, MR>::FLOATS;
-            const float mk = part[MR * HS + row], lk = part[MR * HS + MR + row], mn = fmaxf(m, mk);
-            const float fo = m == -INFINITY ? 0.0f : exp2_fast(m - mn), fk = mk == -INFINITY ? 0.0f : exp2_fast(mk - mn);
-            l = l * fo + lk * fk;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) o[i] = o[i] * fo + part[row * HS + lane + 32 * i] * fk;
-            m = mn;
+    float m, l, o[PER];
+    if (n <= SHARED_PARTS) {
+        for (int row = warp; row < rows; row += JOIN_WARPS) {
+            join_parts<HS, MR>(ends, w, row, n, 0, 1, m, l, o);
+            join_write<HS>(a, q, head, tile * MR + row, m, l, o);
         }
+        return;
+    }
+    for (int row = 0; row < rows; ++row) {
+        join_parts<HS, MR>(ends, w, row, n, warp, JOIN_WARPS, m, l, o);
         if (lane == 0) {
             part_m[warp] = m;
             part_l[warp] = l;
@@ -459,54 +552,56 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const ReadArgs a,
 #pragma unroll
                 for (int i = 0; i < PER; ++i) o[i] += part_o[k][lane + 32 * i] * f;
             }
-            const float inv = l > 0.0f ? 1.0f / l : l;
-            const int mm = tile * MR + row, i = mm / a.group, h = head * a.group + (mm - i * a.group);
-            const int64_t to = (int64_t)(q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride + lane;
-#pragma unroll
-            for (int c = 0; c < PER; ++c) {
-                if (a.bf16_q) static_cast<uint16_t*>(a.out)[to + 32 * c] = bf16_rn_hw(o[c] * inv);
-                else static_cast<float*>(a.out)[to + 32 * c] = o[c] * inv;
-            }
-            if (a.lse && lane == 0) a.lse[(int64_t)(q.start + i) * a.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+            join_write<HS>(a, q, head, tile * MR + row, m, l, o);
         }
         __syncthreads();
     }
 }
 
-constexpr int most_warps(int stage_bytes, int mt) { return mt > 1 ? 8 : stage_bytes <= 2048 ? 16 : stage_bytes <= 4096 ? 12 : stage_bytes <= 8192 ? 8 : 6; }
-constexpr int most_stages(int stage_bytes, int mt) { return 196608 / (most_warps(stage_bytes, mt) * stage_bytes); }
+// Warps of a block: as many as registers allow (eight columns of queries leave room for twelve and more, 32 for eight), and
+// the ring's stages share what is left of 192 KB.
+constexpr int most_warps(int stage_bytes, int nq) { return nq > 2 ? 8 : stage_bytes <= 4096 ? (nq > 1 ? 12 : 16) : stage_bytes <= 8192 ? 8 : 6; }
+constexpr int most_stages(int stage_bytes, int nq) { return 196608 / (most_warps(stage_bytes, nq) * stage_bytes); }
 
-template <typename TS, int L, int HS, int MT>
+template <typename TS, int L, int HS, int NQ>
 cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms) {
-    constexpr int BYTES = Stage<TS, HS>::BYTES, WARPS = most_warps(BYTES, MT), STAGES = most_stages(BYTES, MT), MR = 16 * MT;
+    constexpr int BYTES = Stage<TS, HS>::BYTES, WARPS = most_warps(BYTES, NQ), STAGES = most_stages(BYTES, NQ), MR = 8 * NQ;
     const int workers = sms * WARPS;
     split::Cut* cuts = static_cast<split::Cut*>(room);
     float* ends = reinterpret_cast<float*>(cuts + workers);
-    cudaError_t rc = launch_serving(read_kernel<TS, L, HS, MT, WARPS, STAGES>, dim3(sms), dim3(WARPS * 32), (size_t)WARPS * STAGES * BYTES, st, 1, a, ends, cuts, workers);
+    // by TMA where the store is a tensor for it and 16 keys are one box or two
+    Coming coming{a.s.page_size == 8 ? 8 : a.s.page_size % STEP == 0 ? STEP : 0, 0};
+    CUtensorMap mk = {}, mv = {};
+    PoolShape shape;
+    if (coming.box && (!pool_shape(a.s, &shape) || !pool_map(&mk, a.s.k, a.s.dtype, shape, coming.box) || !pool_map(&mv, a.s.v, a.s.dtype, shape, coming.box))) coming.box = 0;
+    coming.heads_inside = coming.box && shape.heads_inside;
+    cudaError_t rc = launch_serving(read_kernel<TS, L, HS, NQ, WARPS, STAGES>, dim3(sms), dim3(WARPS * 32), (size_t)WARPS * STAGES * BYTES + 1024, st, 1, mk, mv, a, coming, ends,
+                                    cuts, workers);
     if (rc != cudaSuccess) return rc;
     return launch_serving(join_kernel<HS, MR>, dim3(workers), dim3(JOIN_WARPS * 32), 0, st, 1, a, ends, cuts);
 }
 
+template <typename TS, int L, int HS>
+cudaError_t launch_rows(cudaStream_t st, const ReadArgs& a, void* room, int sms) {
+    // Rows per key head that the host expects: a tile of 8, 16 or 32 of them reads the store once (three limbs of 128
+    // channels stay in registers for 16).
+    const int64_t rows = (int64_t)a.max_fresh * a.group;
+    if (rows <= 8) return launch_one<TS, L, HS, 1>(st, a, room, sms);
+    if constexpr (HS < 128 || L == 1)
+        if (rows > 16) return launch_one<TS, L, HS, 4>(st, a, room, sms);
+    return launch_one<TS, L, HS, 2>(st, a, room, sms);
+}
 template <int HS>
 cudaError_t launch_size(cudaStream_t st, const ReadArgs& a, void* room, int sms) {
-    // Rows per key head that the host expects: one tile of 16 reads the store once for up to 16 of them, a tile of 32 for
-    // twice as many (not with f32 queries of 128 channels: their limbs and sums would not stay in registers).
-    const bool wide = (int64_t)a.max_fresh * a.group > 16;
-    if (a.bf16_q) return wide ? launch_one<uint16_t, 1, HS, 2>(st, a, room, sms) : launch_one<uint16_t, 1, HS, 1>(st, a, room, sms);
-    if (a.s.dtype == AVA_BF16) {
-        if constexpr (HS < 128)
-            if (wide) return launch_one<uint16_t, 3, HS, 2>(st, a, room, sms);
-        return launch_one<uint16_t, 3, HS, 1>(st, a, room, sms);
-    }
-    if constexpr (HS < 128)
-        if (wide) return launch_one<float, 3, HS, 2>(st, a, room, sms);
-    return launch_one<float, 3, HS, 1>(st, a, room, sms);
+    if (a.bf16_q) return launch_rows<uint16_t, 1, HS>(st, a, room, sms);
+    if (a.s.dtype == AVA_BF16) return launch_rows<uint16_t, 3, HS>(st, a, room, sms);
+    return launch_rows<float, 3, HS>(st, a, room, sms);
 }
 
 }  // namespace
 
 int64_t paged_read_workspace(int head_size, int sms) {
-    // at most 16 workers on an SM, and at most 256 rows of their tiles (most_warps times 16 or 32)
+    // at most 16 workers on an SM, and at most 256 rows of their tiles (most_warps times 8, 16 or 32; k_pread_tc.cu: 256)
     return (int64_t)sms * 16 * (int64_t)sizeof(split::Cut) + (int64_t)sms * 256 * 2 * (head_size + 2) * 4;
 }
 

@@ -24,6 +24,7 @@
 #include "ava_math.h"
 #include "bf16_hw.cuh"
 #include "kernels.cuh"
+#include "paged_map.cuh"
 #include "read_split.cuh"
 #include "serving.cuh"
 #include "tc_common.cuh"
@@ -176,11 +177,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int page, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
-                 "r"(x), "r"(y), "r"(z), "r"(page), "r"(s32(bar))
-                 : "memory");
-}
 // V as it lies, [key][64 channels] with the 128-byte swizzle, for a multiply that wants it [channel][key]: 64 channels
 // adjacent, 8 keys to 1024 bytes; `group` bytes from one 64-channel column to the next
 __device__ __forceinline__ uint64_t desc_keys_down(uint32_t at, uint32_t group) {
@@ -772,43 +768,13 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const ReadArgs a, const 
     if (a.lse && lane == 0) a.lse[(int64_t)(q.start + i) * a.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
-// A pool as a tensor of [pages][...][...][channels] with the smaller of the head and place strides inside, as long as the
-// strides nest (each a multiple of the one inside it and at least its extent): what a tensor map describes.
-struct Pool {
-    bool heads_inside;
-    uint64_t dims[4], strides[3];
-};
-bool nested(const ava_paged_store& s, Pool* p) {
-    p->heads_inside = s.head_stride <= s.place_stride;
-    const int64_t n1 = p->heads_inside ? s.kv_heads : s.page_size, n2 = p->heads_inside ? s.page_size : s.kv_heads;
-    int64_t s1 = p->heads_inside ? s.head_stride : s.place_stride, s2 = p->heads_inside ? s.place_stride : s.head_stride, s3 = s.page_stride;
-    if (n1 == 1) s1 = s.head_size;     // the stride of a single head or place says nothing
-    if (n2 == 1) s2 = n1 * s1;
-    if (s.n_pages == 1) s3 = n2 * s2;
-    if (s1 < s.head_size || s1 % 8 || s2 < n1 * s1 || s2 % s1 || s3 < n2 * s2 || s3 % s2 || s3 >= (1ll << 39)) return false;
-    const uint64_t d[4] = {(uint64_t)s.head_size, (uint64_t)n1, (uint64_t)n2, (uint64_t)s.n_pages};
-    for (int i = 0; i < 4; ++i) p->dims[i] = d[i];
-    p->strides[0] = (uint64_t)s1 * 2;
-    p->strides[1] = (uint64_t)s2 * 2;
-    p->strides[2] = (uint64_t)s3 * 2;
-    return true;
-}
-bool pool_map(CUtensorMap* map, const void* base, const Pool& p, uint32_t box_rows) {
-    EncodeFn fn = encode_fn();
-    if (!fn) return false;
-    const cuuint64_t dims[4] = {p.dims[0], p.dims[1], p.dims[2], p.dims[3]}, strides[3] = {p.strides[0], p.strides[1], p.strides[2]};
-    const cuuint32_t box[4] = {64, p.heads_inside ? 1u : box_rows, p.heads_inside ? box_rows : 1u, 1}, es[4] = {1, 1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int HS, int L>
-cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, const Pool& pool, bool* taken) {
+cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, const PoolShape& pool, bool* taken) {
     using Sh = Shape<HS, L>;
     const int box_rows = a.s.page_size < KT ? a.s.page_size : KT;
     if (box_rows < 8 || KT % box_rows || a.s.page_size % box_rows) return cudaSuccess;
     CUtensorMap mk, mv;
-    if (!pool_map(&mk, a.s.k, pool, (uint32_t)box_rows) || !pool_map(&mv, a.s.v, pool, (uint32_t)box_rows)) return cudaSuccess;
+    if (!pool_map(&mk, a.s.k, AVA_BF16, pool, box_rows) || !pool_map(&mv, a.s.v, AVA_BF16, pool, box_rows)) return cudaSuccess;
     *taken = true;
     split::Cut* cuts = static_cast<split::Cut*>(room);
     float* ends = reinterpret_cast<float*>(cuts + sms);
@@ -821,8 +787,8 @@ cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, 
 
 cudaError_t launch_paged_read_tc(cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken) {
     *taken = false;
-    Pool pool;
-    if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && !(a.s.head_size == 128 && a.bf16_q)) || (int64_t)a.max_fresh * a.group <= (a.bf16_q ? 32 : 64) || !nested(a.s, &pool))
+    PoolShape pool;
+    if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && !(a.s.head_size == 128 && a.bf16_q)) || (int64_t)a.max_fresh * a.group <= (a.bf16_q ? 32 : 64) || !pool_shape(a.s, &pool))
         return cudaSuccess;
     if (a.s.head_size == 64) return a.bf16_q ? launch_one<64, 1>(st, a, room, sms, pool, taken) : launch_one<64, 3>(st, a, room, sms, pool, taken);
     return launch_one<128, 1>(st, a, room, sms, pool, taken);
