@@ -20,8 +20,9 @@
 #include "ava_math.h"
 #include "bf16_hw.cuh"
 #include "kernels.cuh"
-#include "read_split.cuh"
 #include "paged_map.cuh"
+#include "read_join.cuh"
+#include "read_split.cuh"
 #include "serving.cuh"
 #include "tc_common.cuh"
 
@@ -30,14 +31,8 @@ namespace ava {
 namespace {
 
 constexpr int STEP = 16;                 // keys per stage
-constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 
 using tcc::s32;
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -108,13 +103,6 @@ struct Stage {
 template <int NQ>
 struct Plan {
     static constexpr int MR = 8 * NQ, KT = STEP, START = 2, SNAP = 8;
-};
-
-// Workspace of one worker's piece: the two ends that may be cut (0: goes on from the worker before, 1: goes on in the
-// next), each MR rows of HS sums, then the rows' maxima (of scores times log2 e) and sums.
-template <int HS, int MR>
-struct Ends {
-    static constexpr int FLOATS = MR * (HS + 2);
 };
 
 // How the keys come (box 0: by copies).
@@ -442,9 +430,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const __grid_consta
                 }
             }
         if (!whole && u == it.begin && lane == 0) {
-            cuts[w].r = it.r;
+            cuts[w].start = it.q.start;
             cuts[w].head = it.head;
             cuts[w].tile = it.tile;
+            cuts[w].rows = rows;
             cuts[w].workers = (int)split::last_worker<Pl>(it, per) - w + 1;
         }
         u = run.stop;
@@ -457,81 +446,28 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const __grid_consta
     if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
 }
 
-// Joins the ends of the stretches that were cut: one block per worker, idle unless a cut stretch begins in its piece.
-// With the parts' maxima m_i, sums l_i and mixes o_i: m = max m_i, out = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
-// A warp takes a row: the parts' maxima and sums a lane each, then all lanes the parts' mixes, whose loads depend on nothing
-// but the weights.  Stretches of many parts (a long sequence) have the block's warps share a row's parts.
+// Joins the ends of the stretches that were cut (read_join.cuh): one block per worker, idle unless a cut stretch begins in its
+// piece.  A warp takes a row; stretches of many parts (a long sequence) have the block's warps share a row's parts.
 constexpr int JOIN_WARPS = 8, SHARED_PARTS = 16;
-
-// the parts k = k0, k0 + step, ... < n of a row: their common maximum, sum and mix
-template <int HS, int MR>
-__device__ __forceinline__ void join_parts(const float* ends, int w, int row, int n, int k0, int step, float& m, float& l, float (&o)[HS / 32]) {
-    constexpr int PER = HS / 32;
-    const int lane = threadIdx.x & 31;
-    m = -INFINITY;
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = 0.0f;
-    for (int b = k0; b < n; b += 32 * step) {
-        const int mine = b + lane * step;
-        auto part_of = [&](int k) { return ends + ((int64_t)(w + k) * 2 + (k == 0 ? 1 : 0)) * Ends<HS, MR>::FLOATS; };
-        const float mk = mine < n ? part_of(mine)[MR * HS + row] : -INFINITY, lk = mine < n ? part_of(mine)[MR * HS + MR + row] : 0.0f;
-        float now = mk;
-#pragma unroll
-        for (int x = 16; x; x >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, x));
-        now = fmaxf(now, m);
-        const float before = m == -INFINITY ? 0.0f : exp2_fast(m - now), weight = mk == -INFINITY ? 0.0f : exp2_fast(mk - now);
-        float s = lk * weight;
-#pragma unroll
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        l = l * before + s;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) o[i] *= before;
-        const int count = min(32, (n - b + step - 1) / step);
-#pragma unroll 4
-        for (int k = 0; k < count; ++k) {
-            const float wk = __shfl_sync(0xffffffffu, weight, k);
-            const float* part = part_of(b + k * step) + row * HS + lane;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) o[i] = fmaf(part[32 * i], wk, o[i]);
-        }
-        m = now;
-    }
-}
-template <int HS>
-__device__ __forceinline__ void join_write(const ReadArgs& a, const split::Request& q, int head, int m_row, float m, float l, const float (&o)[HS / 32]) {
-    const int lane = threadIdx.x & 31;
-    const float inv = l > 0.0f ? 1.0f / l : l;
-    const int i = m_row / a.group, h = head * a.group + (m_row - i * a.group);
-    const int64_t to = (int64_t)(q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride + lane;
-#pragma unroll
-    for (int c = 0; c < HS / 32; ++c) {
-        if (a.bf16_q) static_cast<uint16_t*>(a.out)[to + 32 * c] = bf16_rn_hw(o[c] * inv);
-        else static_cast<float*>(a.out)[to + 32 * c] = o[c] * inv;
-    }
-    if (a.lse && lane == 0) a.lse[(int64_t)(q.start + i) * a.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
-}
-
 template <int HS, int MR>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const ReadArgs a, const float* __restrict__ ends, const split::Cut* __restrict__ cuts) {
     pdl_enter();
-    const int w = blockIdx.x, n = cuts[w].workers;
+    const int w = blockIdx.x;
+    const split::Cut cut = cuts[w];
+    const int n = cut.workers;
     if (n == 0) return;
     constexpr int PER = HS / 32;
     __shared__ float part_o[JOIN_WARPS][HS], part_m[JOIN_WARPS], part_l[JOIN_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    bool bad = false;
-    const split::Request q = split::request(a, cuts[w].r, &bad);
-    const int head = cuts[w].head, tile = cuts[w].tile, rows = min(q.f * a.group - tile * MR, MR);
     float m, l, o[PER];
     if (n <= SHARED_PARTS) {
-        for (int row = warp; row < rows; row += JOIN_WARPS) {
+        for (int row = warp; row < cut.rows; row += JOIN_WARPS) {
             join_parts<HS, MR>(ends, w, row, n, 0, 1, m, l, o);
-            join_write<HS>(a, q, head, tile * MR + row, m, l, o);
+            join_write<HS>(a, cut.start, cut.head, cut.tile * MR + row, m, l, o);
         }
         return;
     }
-    for (int row = 0; row < rows; ++row) {
+    for (int row = 0; row < cut.rows; ++row) {
         join_parts<HS, MR>(ends, w, row, n, warp, JOIN_WARPS, m, l, o);
         if (lane == 0) {
             part_m[warp] = m;
@@ -552,15 +488,15 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const ReadArgs a,
 #pragma unroll
                 for (int i = 0; i < PER; ++i) o[i] += part_o[k][lane + 32 * i] * f;
             }
-            join_write<HS>(a, q, head, tile * MR + row, m, l, o);
+            join_write<HS>(a, cut.start, cut.head, cut.tile * MR + row, m, l, o);
         }
         __syncthreads();
     }
 }
 
-// Warps of a block: as many as registers allow (eight columns of queries leave room for twelve and more, 32 for eight), and
+// Warps of a block: as many as registers allow (16 columns of queries leave room for twelve, 32 for eight; 16 warps with three stages each were slower), and
 // the ring's stages share what is left of 192 KB.
-constexpr int most_warps(int stage_bytes, int nq) { return nq > 2 ? 8 : stage_bytes <= 4096 ? (nq > 1 ? 12 : 16) : stage_bytes <= 8192 ? 8 : 6; }
+constexpr int most_warps(int stage_bytes, int nq) { return nq > 2 ? 8 : stage_bytes <= 4096 ? 12 : stage_bytes <= 8192 ? 8 : 6; }
 constexpr int most_stages(int stage_bytes, int nq) { return 196608 / (most_warps(stage_bytes, nq) * stage_bytes); }
 
 template <typename TS, int L, int HS, int NQ>
@@ -587,8 +523,10 @@ cudaError_t launch_rows(cudaStream_t st, const ReadArgs& a, void* room, int sms)
     // channels stay in registers for 16).
     const int64_t rows = (int64_t)a.max_fresh * a.group;
     if (rows <= 8) return launch_one<TS, L, HS, 1>(st, a, room, sms);
-    if constexpr (HS < 128 || L == 1)
-        if (rows > 16) return launch_one<TS, L, HS, 4>(st, a, room, sms);
+    if constexpr (HS < 128 || L == 1) {
+        if (rows > 24) return launch_one<TS, L, HS, 4>(st, a, room, sms);
+        if (rows > 16) return launch_one<TS, L, HS, 3>(st, a, room, sms);
+    }
     return launch_one<TS, L, HS, 2>(st, a, room, sms);
 }
 template <int HS>

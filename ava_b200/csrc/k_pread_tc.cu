@@ -25,6 +25,7 @@
 #include "bf16_hw.cuh"
 #include "kernels.cuh"
 #include "paged_map.cuh"
+#include "read_join.cuh"
 #include "read_split.cuh"
 #include "serving.cuh"
 #include "tc_common.cuh"
@@ -41,7 +42,6 @@ struct Plan {                            // of the line: a tile's queries and re
     static constexpr int MR = 256, KT = 64, START = 4, SNAP = 4;
 };
 constexpr int MR = Plan::MR, KT = Plan::KT;
-constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by before the sums are rescaled
 
 template <int HS_, int L_>
@@ -64,11 +64,6 @@ struct Shape {
     static_assert(BYTES <= 232448, "shared memory");
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -514,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             tc_after();
             {
                 const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum) : 1.0f;
-                float* end_of = ends + ((int64_t)worker * 2 + (u == it.begin ? 1 : 0)) * (MR * (HS + 2));
+                float* end_of = ends + ((int64_t)worker * 2 + (u == it.begin ? 1 : 0)) * Ends<HS, MR>::FLOATS;
                 const int64_t to = (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride;
 #pragma unroll(FLUSH ? HS / 32 : 1)
                 for (int c = 0; c < HS; c += 32) {
@@ -576,9 +571,10 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     }
                 }
                 if (!whole && u == it.begin && tid == 0) {
-                    cuts[worker].r = it.r;
+                    cuts[worker].start = it.q.start;
                     cuts[worker].head = it.head;
                     cuts[worker].tile = it.tile;
+                    cuts[worker].rows = run.rows;
                     cuts[worker].workers = (int)split::last_worker<Plan>(it, per) - worker + 1;
                 }
             }
@@ -734,38 +730,16 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
     if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// Joins the ends of the stretches that were cut (see k_pread.cu): a block per worker and eight rows, a warp per row.
+// Joins the ends of the stretches that were cut (read_join.cuh): a block per worker and eight rows, a warp per row.
 template <int HS>
 __global__ void __launch_bounds__(256) join_rows_kernel(const ReadArgs a, const float* __restrict__ ends, const split::Cut* __restrict__ cuts) {
     pdl_enter();
-    const int w = blockIdx.x, n = cuts[w].workers, lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (n == 0) return;
-    constexpr int PER = HS / 32;
-    bool bad = false;
-    const split::Request q = split::request(a, cuts[w].r, &bad);
-    const int head = cuts[w].head, tile = cuts[w].tile;
-    if (row >= min(q.f * a.group - tile * MR, MR)) return;
-    float m = -INFINITY, l = 0.0f, o[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = 0.0f;
-    for (int k = 0; k < n; ++k) {
-        const float* part = ends + ((int64_t)(w + k) * 2 + (k == 0 ? 1 : 0)) * (MR * (HS + 2));
-        const float mk = part[MR * HS + row], lk = part[MR * HS + MR + row], mn = fmaxf(m, mk);
-        const float fo = m == -INFINITY ? 0.0f : exp2_fast(m - mn), fk = mk == -INFINITY ? 0.0f : exp2_fast(mk - mn);
-        l = l * fo + lk * fk;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) o[i] = o[i] * fo + part[row * HS + lane + 32 * i] * fk;
-        m = mn;
-    }
-    const float inv = l > 0.0f ? 1.0f / l : l;
-    const int mm = tile * MR + row, i = mm / a.group, h = head * a.group + (mm - i * a.group);
-    const int64_t to = (int64_t)(q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride + lane;
-#pragma unroll
-    for (int c = 0; c < PER; ++c) {
-        if (a.bf16_q) static_cast<uint16_t*>(a.out)[to + 32 * c] = bf16_rn_hw(o[c] * inv);
-        else static_cast<float*>(a.out)[to + 32 * c] = o[c] * inv;
-    }
-    if (a.lse && lane == 0) a.lse[(int64_t)(q.start + i) * a.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+    const split::Cut cut = cuts[blockIdx.x];
+    const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (cut.workers == 0 || row >= cut.rows) return;
+    float m, l, o[HS / 32];
+    join_parts<HS, MR>(ends, blockIdx.x, row, cut.workers, 0, 1, m, l, o);
+    join_write<HS>(a, cut.start, cut.head, cut.tile * MR + row, m, l, o);
 }
 
 template <int HS, int L>

@@ -229,9 +229,10 @@ __device__ __forceinline__ long long last_worker(const Item& it, long long per) 
 }
 
 // What the joining kernel is told by the worker in whose piece a cut stretch begins.
-struct Cut {
-    int r, head, tile;
+struct __align__(16) Cut {
     int workers;                // how many workers' pieces the stretch runs through; 0: this worker begins none
+    int start, head, tile, rows;   // the request's first packed token, the key head, the tile and its rows
+    int unused[3];
 };
 
 }  // namespace split
