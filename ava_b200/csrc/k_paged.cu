@@ -353,14 +353,14 @@ __global__ void __launch_bounds__(256) append_any_kernel(const AppendArgs a) {
 
 }  // namespace
 
-cudaError_t launch_paged_plan(cudaStream_t st, const PlanArgs& a) {
+cudaError_t launch_paged_plan(int device, cudaStream_t st, const PlanArgs& a) {
     const bool one = a.max_tokens <= PER_THREAD * PLAN_THREADS;   // one round of the one block
-    cudaError_t rc = launch_serving(plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, 1, a, one ? 1 : 0);
+    cudaError_t rc = launch_serving<plan_kernel>(device, dim3(1), dim3(PLAN_THREADS), 0, st, 1, a, one ? 1 : 0);
     if (rc != cudaSuccess || one) return rc;
-    return launch_serving(plan_tokens_kernel, dim3((a.max_tokens + TOKENS_PER_BLOCK - 1) / TOKENS_PER_BLOCK), dim3(TOKEN_THREADS), 0, st, 1, a);
+    return launch_serving<plan_tokens_kernel>(device, dim3((a.max_tokens + TOKENS_PER_BLOCK - 1) / TOKENS_PER_BLOCK), dim3(TOKEN_THREADS), 0, st, 1, a);
 }
 
-cudaError_t launch_paged_append(cudaStream_t st, const AppendArgs& a) {
+cudaError_t launch_paged_append(int device, cudaStream_t st, const AppendArgs& a) {
     const int in = a.bf16_in ? 2 : 4, out = a.s.dtype == AVA_BF16 ? 2 : 4;
     const uintptr_t pointers = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.s.k) | reinterpret_cast<uintptr_t>(a.s.v);
     const int64_t bytes = a.token_stride * in | a.head_stride * in | a.s.page_stride * out | a.s.head_stride * out | a.s.place_stride * out;
@@ -369,14 +369,14 @@ cudaError_t launch_paged_append(cudaStream_t st, const AppendArgs& a) {
         // few tokens are spread over the SMs first (a piece per thread); many go four to a thread
         const int64_t threads = n / 8 <= 148 * 1024 ? n / 8 : (n / 8 + 3) / 4;
         const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
-        if (a.bf16_in) return launch_serving(append_kernel<true, true>, grid, block, 0, st, 1, a);
-        if (out == 2) return launch_serving(append_kernel<false, true>, grid, block, 0, st, 1, a);
-        return launch_serving(append_kernel<false, false>, grid, block, 0, st, 1, a);
+        if (a.bf16_in) return launch_serving<append_kernel<true, true>>(device, grid, block, 0, st, 1, a);
+        if (out == 2) return launch_serving<append_kernel<false, true>>(device, grid, block, 0, st, 1, a);
+        return launch_serving<append_kernel<false, false>>(device, grid, block, 0, st, 1, a);
     }
     const dim3 grid((unsigned)((n + 255) / 256 < 148 * 64 ? (n + 255) / 256 : 148 * 64)), block(256);
-    if (a.bf16_in) return launch_serving(append_any_kernel<uint16_t, uint16_t>, grid, block, 0, st, 1, a);
-    if (out == 2) return launch_serving(append_any_kernel<float, uint16_t>, grid, block, 0, st, 1, a);
-    return launch_serving(append_any_kernel<float, float>, grid, block, 0, st, 1, a);
+    if (a.bf16_in) return launch_serving<append_any_kernel<uint16_t, uint16_t>>(device, grid, block, 0, st, 1, a);
+    if (out == 2) return launch_serving<append_any_kernel<float, uint16_t>>(device, grid, block, 0, st, 1, a);
+    return launch_serving<append_any_kernel<float, float>>(device, grid, block, 0, st, 1, a);
 }
 
 }  // namespace ava

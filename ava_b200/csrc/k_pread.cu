@@ -500,7 +500,7 @@ constexpr int most_warps(int stage_bytes, int nq) { return nq > 2 ? 8 : stage_by
 constexpr int most_stages(int stage_bytes, int nq) { return 196608 / (most_warps(stage_bytes, nq) * stage_bytes); }
 
 template <typename TS, int L, int HS, int NQ>
-cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms) {
+cudaError_t launch_one(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms) {
     constexpr int BYTES = Stage<TS, HS>::BYTES, WARPS = most_warps(BYTES, NQ), STAGES = most_stages(BYTES, NQ), MR = 8 * NQ;
     const int workers = sms * WARPS;
     split::Cut* cuts = static_cast<split::Cut*>(room);
@@ -511,29 +511,29 @@ cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms) 
     PoolShape shape;
     if (coming.box && (!pool_shape(a.s, &shape) || !pool_map(&mk, a.s.k, a.s.dtype, shape, coming.box) || !pool_map(&mv, a.s.v, a.s.dtype, shape, coming.box))) coming.box = 0;
     coming.heads_inside = coming.box && shape.heads_inside;
-    cudaError_t rc = launch_serving(read_kernel<TS, L, HS, NQ, WARPS, STAGES>, dim3(sms), dim3(WARPS * 32), (size_t)WARPS * STAGES * BYTES + 1024, st, 1, mk, mv, a, coming, ends,
+    cudaError_t rc = launch_serving<read_kernel<TS, L, HS, NQ, WARPS, STAGES>>(device, dim3(sms), dim3(WARPS * 32), (size_t)WARPS * STAGES * BYTES + 1024, st, 1, mk, mv, a, coming, ends,
                                     cuts, workers);
     if (rc != cudaSuccess) return rc;
-    return launch_serving(join_kernel<HS, MR>, dim3(workers), dim3(JOIN_WARPS * 32), 0, st, 1, a, ends, cuts);
+    return launch_serving<join_kernel<HS, MR>>(device, dim3(workers), dim3(JOIN_WARPS * 32), 0, st, 1, a, ends, cuts);
 }
 
 template <typename TS, int L, int HS>
-cudaError_t launch_rows(cudaStream_t st, const ReadArgs& a, void* room, int sms) {
+cudaError_t launch_rows(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms) {
     // Rows per key head that the host expects: a tile of 8, 16 or 32 of them reads the store once (three limbs of 128
     // channels stay in registers for 16).
     const int64_t rows = (int64_t)a.max_fresh * a.group;
-    if (rows <= 8) return launch_one<TS, L, HS, 1>(st, a, room, sms);
+    if (rows <= 8) return launch_one<TS, L, HS, 1>(device, st, a, room, sms);
     if constexpr (HS < 128 || L == 1) {
-        if (rows > 24) return launch_one<TS, L, HS, 4>(st, a, room, sms);
-        if (rows > 16) return launch_one<TS, L, HS, 3>(st, a, room, sms);
+        if (rows > 24) return launch_one<TS, L, HS, 4>(device, st, a, room, sms);
+        if (rows > 16) return launch_one<TS, L, HS, 3>(device, st, a, room, sms);
     }
-    return launch_one<TS, L, HS, 2>(st, a, room, sms);
+    return launch_one<TS, L, HS, 2>(device, st, a, room, sms);
 }
 template <int HS>
-cudaError_t launch_size(cudaStream_t st, const ReadArgs& a, void* room, int sms) {
-    if (a.bf16_q) return launch_rows<uint16_t, 1, HS>(st, a, room, sms);
-    if (a.s.dtype == AVA_BF16) return launch_rows<uint16_t, 3, HS>(st, a, room, sms);
-    return launch_rows<float, 3, HS>(st, a, room, sms);
+cudaError_t launch_size(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms) {
+    if (a.bf16_q) return launch_rows<uint16_t, 1, HS>(device, st, a, room, sms);
+    if (a.s.dtype == AVA_BF16) return launch_rows<uint16_t, 3, HS>(device, st, a, room, sms);
+    return launch_rows<float, 3, HS>(device, st, a, room, sms);
 }
 
 }  // namespace
@@ -543,13 +543,13 @@ int64_t paged_read_workspace(int head_size, int sms) {
     return (int64_t)sms * 16 * (int64_t)sizeof(split::Cut) + (int64_t)sms * 256 * 2 * (head_size + 2) * 4;
 }
 
-cudaError_t launch_paged_read(cudaStream_t st, const ReadArgs& a, void* room, int sms) {
+cudaError_t launch_paged_read(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms) {
     bool taken = false;
-    const cudaError_t rc = launch_paged_read_tc(st, a, room, sms, &taken);
+    const cudaError_t rc = launch_paged_read_tc(device, st, a, room, sms, &taken);
     if (taken || rc != cudaSuccess) return rc;
-    if (a.s.head_size == 32) return launch_size<32>(st, a, room, sms);
-    if (a.s.head_size == 64) return launch_size<64>(st, a, room, sms);
-    return launch_size<128>(st, a, room, sms);
+    if (a.s.head_size == 32) return launch_size<32>(device, st, a, room, sms);
+    if (a.s.head_size == 64) return launch_size<64>(device, st, a, room, sms);
+    return launch_size<128>(device, st, a, room, sms);
 }
 
 }  // namespace ava

@@ -743,7 +743,7 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const ReadArgs a, const 
 }
 
 template <int HS, int L>
-cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, const PoolShape& pool, bool* taken) {
+cudaError_t launch_one(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms, const PoolShape& pool, bool* taken) {
     using Sh = Shape<HS, L>;
     const int box_rows = a.s.page_size < KT ? a.s.page_size : KT;
     if (box_rows < 8 || KT % box_rows || a.s.page_size % box_rows) return cudaSuccess;
@@ -752,20 +752,20 @@ cudaError_t launch_one(cudaStream_t st, const ReadArgs& a, void* room, int sms, 
     *taken = true;
     split::Cut* cuts = static_cast<split::Cut*>(room);
     float* ends = reinterpret_cast<float*>(cuts + sms);
-    cudaError_t rc = launch_serving(read_tc_kernel<Sh>, dim3(sms), dim3(THREADS), Sh::BYTES, st, 1, mk, mv, a, pool.heads_inside ? 1 : 0, box_rows, ends, cuts);
+    cudaError_t rc = launch_serving<read_tc_kernel<Sh>>(device, dim3(sms), dim3(THREADS), Sh::BYTES, st, 1, mk, mv, a, pool.heads_inside ? 1 : 0, box_rows, ends, cuts);
     if (rc != cudaSuccess) return rc;
-    return launch_serving(join_rows_kernel<HS>, dim3(sms, MR / 8), dim3(256), 0, st, 1, a, ends, cuts);
+    return launch_serving<join_rows_kernel<HS>>(device, dim3(sms, MR / 8), dim3(256), 0, st, 1, a, ends, cuts);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_read_tc(cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken) {
+cudaError_t launch_paged_read_tc(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken) {
     *taken = false;
     PoolShape pool;
     if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && !(a.s.head_size == 128 && a.bf16_q)) || (int64_t)a.max_fresh * a.group <= (a.bf16_q ? 32 : 64) || !pool_shape(a.s, &pool))
         return cudaSuccess;
-    if (a.s.head_size == 64) return a.bf16_q ? launch_one<64, 1>(st, a, room, sms, pool, taken) : launch_one<64, 3>(st, a, room, sms, pool, taken);
-    return launch_one<128, 1>(st, a, room, sms, pool, taken);
+    if (a.s.head_size == 64) return a.bf16_q ? launch_one<64, 1>(device, st, a, room, sms, pool, taken) : launch_one<64, 3>(device, st, a, room, sms, pool, taken);
+    return launch_one<128, 1>(device, st, a, room, sms, pool, taken);
 }
 
 }  // namespace ava

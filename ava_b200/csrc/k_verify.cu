@@ -22,7 +22,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int V_THREADS = 512, V_WARPS = V_THREADS / 32, V_TILES = 64;
+constexpr int V_THREADS = 256, V_WARPS = V_THREADS / 32, V_TILES = 32, V_PARTS = 8;
 
 struct Row {
     const float *p, *q;   // q nullptr: p alone
@@ -62,14 +62,14 @@ __device__ __forceinline__ void weights4(const Row& w, int j, const float (&p)[4
 
 // The block's part [lo, hi) in tiles of 128 * m tokens: their sums.  A warp walks its V_TILES / V_WARPS tiles together, so
 // that their loads are in flight at once (one tile after the other waited for memory tile by tile: 63 us for 256 requests
-// of 32768 tokens).
+// of 32768 tokens; 512 threads of 128 registers, one block to an SM and so wave after wave: 37 us).
 __device__ __forceinline__ void tile_sums(const Row& w, int lo, int hi, int m, bool wide, double* sums) {
     constexpr int MINE = V_TILES / V_WARPS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double s[MINE];
 #pragma unroll
     for (int k = 0; k < MINE; ++k) s[k] = 0.0;
-#pragma unroll 2
+#pragma unroll 1
     for (int b = 0; b < m; ++b) {
         float p[MINE][4], q[MINE][4];
 #pragma unroll
@@ -90,13 +90,13 @@ __device__ __forceinline__ void tile_sums(const Row& w, int lo, int hi, int m, b
         for (int k = 0; k < MINE; ++k) sums[warp * MINE + k] = s[k];
 }
 
-__global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(V_THREADS, 4) verify_kernel(const VerifyArgs a) {
     pdl_enter();
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
     const int r = blockIdx.x / parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     __shared__ double sums[V_TILES];
-    __shared__ double total;            // of this block's part; read by the others of the cluster
+    __shared__ double totals[2][V_PARTS];   // of every block's part, written by that block; once more after a fall back
     __shared__ int s_kept, s_pick;
     __shared__ float best_x[V_WARPS];
     __shared__ int best_i[V_WARPS];
@@ -211,21 +211,21 @@ __global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
         tile_sums(w, lo, hi, m, wide, sums);
         __syncthreads();
         if (warp == 0) {
-            double s = sums[lane] + sums[lane + 32];
+            double s = sums[lane];
 #pragma unroll
             for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (lane == 0) total = s;
+            if (lane < parts) *cluster.map_shared_rank(&totals[attempt][part], lane) = s;
         }
-        cluster.sync();
+        cluster.sync();   // after it a block reads its own memory only, so the others may leave
         whole = 0.0;
-        for (int k = 0; k < parts; ++k) whole += *cluster.map_shared_rank(&total, k);
+        for (int k = 0; k < parts; ++k) whole += totals[attempt][k];
         // the part the drawn place lies in: the first whose running sum exceeds u * whole, else the last with any mass
         const double target = u * whole;
         double run = 0.0;
         bool found = false;
         mine = -1;
         for (int k = 0; k < parts && !found; ++k) {
-            const double s = *cluster.map_shared_rank(&total, k);
+            const double s = totals[attempt][k];
             if (s > 0.0) {
                 mine = k;
                 before = run;
@@ -233,7 +233,6 @@ __global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
             run += s;
             found = run > target;
         }
-        cluster.sync();   // nobody leaves, or sums again, while its total is still read
         if ((whole > 0.0 && whole < INFINITY) || (!w.q && w.without < 0)) break;
         w.q = nullptr;    // no mass in the difference: the target's own
         w.without = -1;
@@ -243,22 +242,17 @@ __global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
     const double target = u * whole;
     if (mass && warp == 0) {
         // the tile, then the token: by running sums over lanes, in token order
-        const double s0 = sums[2 * lane], s1 = sums[2 * lane + 1];
-        double inc = s0 + s1;
+        const double own = sums[lane];
+        double inc = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double y = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += y;
         }
-        const double b0 = before + (inc - (s0 + s1)), b1 = b0 + s0;
-        int tile = -1;
-        double at = 0.0;
-        const unsigned over = __ballot_sync(0xffffffffu, before + inc > target && s0 + s1 > 0.0);
-        const unsigned some = __ballot_sync(0xffffffffu, s0 + s1 > 0.0);
-        const int who = over ? __ffs(over) - 1 : 31 - __clz(some);
-        const bool second = !(s0 > 0.0) || (s1 > 0.0 && !(b1 > target));
-        tile = __shfl_sync(0xffffffffu, 2 * lane + (second ? 1 : 0), who);
-        at = __shfl_sync(0xffffffffu, second ? b1 : b0, who);
+        const unsigned over = __ballot_sync(0xffffffffu, before + inc > target && own > 0.0);
+        const unsigned some = __ballot_sync(0xffffffffu, own > 0.0);
+        const int tile = over ? __ffs(over) - 1 : 31 - __clz(some);
+        double at = __shfl_sync(0xffffffffu, before + (inc - own), tile);
         const bool wide = !((reinterpret_cast<uintptr_t>(w.p) | reinterpret_cast<uintptr_t>(w.q)) & 15);
         int pick = -1, last = -1;
         for (int b = 0; b < m && pick < 0; ++b) {
@@ -267,14 +261,14 @@ __global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
             double x[4];
             load4(w, j, hi, wide, p, q);
             weights4(w, j, p, q, x);
-            const double own = ((x[0] + x[1]) + x[2]) + x[3];
-            double sum = own;
+            const double four = ((x[0] + x[1]) + x[2]) + x[3];
+            double sum = four;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const double y = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += y;
             }
-            double run = at + (sum - own);
+            double run = at + (sum - four);
             int first = -1, some_here = -1;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -301,12 +295,12 @@ __global__ void __launch_bounds__(V_THREADS) verify_kernel(const VerifyArgs a) {
 
 }  // namespace
 
-cudaError_t launch_verify(cudaStream_t st, const VerifyArgs& a) {
+cudaError_t launch_verify(int device, cudaStream_t st, const VerifyArgs& a) {
     // blocks per request: enough to have about four on every SM (one request's row is then read by eight SMs), one for
     // the larger batches, whose requests fill the GPU by themselves
-    int cluster = 8;
+    int cluster = V_PARTS;
     while (cluster > 1 && (int64_t)a.rows * cluster > 4 * 148) cluster >>= 1;
-    return launch_serving(verify_kernel, dim3(a.rows * cluster), dim3(V_THREADS), 0, st, cluster, a);
+    return launch_serving<verify_kernel>(device, dim3(a.rows * cluster), dim3(V_THREADS), 0, st, cluster, a);
 }
 
 }  // namespace ava

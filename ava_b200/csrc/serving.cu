@@ -3,8 +3,8 @@
 // thread-local string.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
-#include <exception>
 #include <string>
 
 #include "../../include/ava_engine.h"
@@ -24,16 +24,25 @@ int fail(int code, const char* call, const char* why) noexcept {
     return code;
 }
 
+// Devices of this process (their number does not change once there are any).
+int device_count() {
+    static std::atomic<int> known{0};
+    int n = known.load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    if (cudaGetDeviceCount(&n) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    known.store(n, std::memory_order_relaxed);
+    return n;
+}
+
 // The call's device for as long as it lives; the thread's own comes back.
 struct OnDevice {
     int before = -1;
     bool ok = false;
     explicit OnDevice(int device) {
-        int count = 0;
-        if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count) {
-            cudaGetLastError();
-            return;
-        }
+        if (device < 0 || device >= device_count()) return;
         if (cudaGetDevice(&before) != cudaSuccess) return;
         ok = before == device || cudaSetDevice(device) == cudaSuccess;
         if (before == device) before = -1;
@@ -96,7 +105,7 @@ int ava_paged_plan(int device, void* stream, const int32_t* cached, const int32_
     a.table = table; a.owned_out = owned_out; a.free_list = free_list; a.free_count_out = free_count_out; a.q_start = q_start;
     a.slot = slot; a.pos = pos; a.row = row; a.status = status;
     a.rows = rows; a.page_size = page_size; a.n_pages = n_pages; a.max_pages = max_pages; a.max_tokens = max_tokens; a.trim = trim != 0;
-    return launched(launch_paged_plan(static_cast<cudaStream_t>(stream), a), call);
+    return launched(launch_paged_plan(device, static_cast<cudaStream_t>(stream), a), call);
 }
 
 int ava_paged_append(int device, void* stream, const ava_paged_store* store, const void* k, const void* v, int32_t dtype, int64_t token_stride,
@@ -117,7 +126,7 @@ int ava_paged_append(int device, void* stream, const ava_paged_store* store, con
     AppendArgs a{};
     a.s = *store; a.k = k; a.v = v; a.token_stride = token_stride; a.head_stride = head_stride; a.slot = slot; a.status = status;
     a.tokens = tokens; a.bf16_in = dtype == AVA_BF16;
-    return launched(launch_paged_append(static_cast<cudaStream_t>(stream), a), call);
+    return launched(launch_paged_append(device, static_cast<cudaStream_t>(stream), a), call);
 }
 
 int64_t ava_paged_attend_workspace(int device, int32_t head_size) {
@@ -166,7 +175,7 @@ int ava_paged_attend(int device, void* stream, const ava_paged_store* store, con
     a.table = table; a.cached = cached; a.first = first; a.q_start = q_start; a.status = status; a.scale = scale;
     a.heads = heads; a.group = heads / store->kv_heads; a.max_pages = max_pages; a.rows = rows; a.max_tokens = max_tokens; a.max_fresh = max_fresh;
     a.window = window; a.bf16_q = dtype == AVA_BF16;
-    return launched(launch_paged_read(static_cast<cudaStream_t>(stream), a, workspace, sms), call);
+    return launched(launch_paged_read(device, static_cast<cudaStream_t>(stream), a, workspace, sms), call);
 }
 
 int ava_verify_drafts(int device, void* stream, const float* p, int64_t p_stride, const float* q, int64_t q_stride, const uint32_t* tok,
@@ -187,7 +196,7 @@ int ava_verify_drafts(int device, void* stream, const float* p, int64_t p_stride
     VerifyArgs a{};
     a.p = p; a.q = q; a.p_stride = p_stride; a.q_stride = q_stride; a.tok = tok; a.q_start = q_start; a.uniform = uniform; a.out = out; a.n_out = n_out;
     a.status = status; a.rows = rows; a.max_tokens = max_tokens; a.vocab = vocab; a.max_out = max_out;
-    return launched(launch_verify(static_cast<cudaStream_t>(stream), a), call);
+    return launched(launch_verify(device, static_cast<cudaStream_t>(stream), a), call);
 }
 
 }  // extern "C"

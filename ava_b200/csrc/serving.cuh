@@ -4,18 +4,23 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/ava_engine.h"
 
 namespace ava {
 
-// One launch with programmatic dependent launch (the kernels start with pdl_enter, kernels.cuh).  Unlike launch_k it
-// shares nothing between threads: these operators may be called from several threads at once.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_serving(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
-    if (smem > 48 * 1024) {
-        const cudaError_t rc = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (rc != cudaSuccess) return rc;
-    }
+inline cudaError_t launch_as(void (*kernel)(KArgs...), const cudaLaunchConfig_t& cfg, Args&&... args) {
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// One launch with programmatic dependent launch (the kernels start with pdl_enter, kernels.cuh).  Unlike launch_k it
+// shares nothing between threads but a word per kernel that says on which devices its shared memory has been asked for:
+// these operators may be called from several threads at once.
+template <auto Kernel, typename... Args>
+inline cudaError_t launch_serving(int device, dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
+    static std::atomic<uint64_t> asked{0};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -30,7 +35,13 @@ inline cudaError_t launch_serving(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+    const uint64_t bit = 1ull << (device & 63);
+    if (smem > 48 * 1024 && (device > 63 || !(asked.load(std::memory_order_relaxed) & bit))) {
+        const cudaError_t rc = cudaFuncSetAttribute(reinterpret_cast<const void*>(Kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (rc != cudaSuccess) return rc;
+        asked.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return launch_as(Kernel, cfg, static_cast<Args&&>(args)...);
 }
 
 // ---- the step's lists (k_paged.cu)
@@ -42,7 +53,7 @@ struct PlanArgs {
     uint32_t* status;
     int rows, page_size, n_pages, max_pages, max_tokens, trim;
 };
-cudaError_t launch_paged_plan(cudaStream_t st, const PlanArgs& a);
+cudaError_t launch_paged_plan(int device, cudaStream_t st, const PlanArgs& a);
 
 // ---- new keys and values into their pages (k_paged.cu)
 struct AppendArgs {
@@ -53,7 +64,7 @@ struct AppendArgs {
     uint32_t* status;
     int tokens, bf16_in;
 };
-cudaError_t launch_paged_append(cudaStream_t st, const AppendArgs& a);
+cudaError_t launch_paged_append(int device, cudaStream_t st, const AppendArgs& a);
 
 // ---- the read (k_pread.cu)
 struct ReadArgs {
@@ -68,10 +79,10 @@ struct ReadArgs {
     int heads, group, max_pages, rows, max_tokens, max_fresh, window, bf16_q;
 };
 // room: paged_read_workspace bytes
-cudaError_t launch_paged_read(cudaStream_t st, const ReadArgs& a, void* room, int sms);
+cudaError_t launch_paged_read(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms);
 int64_t paged_read_workspace(int head_size, int sms);
 // the same on tcgen05 (k_pread_tc.cu); *taken false: not its case, nothing was queued
-cudaError_t launch_paged_read_tc(cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken);
+cudaError_t launch_paged_read_tc(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken);
 
 // ---- drafted tokens (k_verify.cu)
 struct VerifyArgs {
@@ -85,6 +96,6 @@ struct VerifyArgs {
     uint32_t* status;
     int rows, max_tokens, vocab, max_out;
 };
-cudaError_t launch_verify(cudaStream_t st, const VerifyArgs& a);
+cudaError_t launch_verify(int device, cudaStream_t st, const VerifyArgs& a);
 
 }  // namespace ava
