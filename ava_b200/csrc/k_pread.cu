@@ -87,6 +87,17 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     return y;
 }
 
+// a word of f32, or of two bf16: whether any of it is not finite, and the word with that part 0
+template <bool F32>
+__device__ __forceinline__ bool not_finite(uint32_t x) {
+    return (x & 0x7f800000u) == 0x7f800000u || (!F32 && (x & 0x7f80u) == 0x7f80u);
+}
+template <bool F32>
+__device__ __forceinline__ uint32_t finite_only(uint32_t x) {
+    if (F32) return not_finite<true>(x) ? 0u : x;
+    return x & ~(((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u));
+}
+
 // How a warp lays out its stage: K, then V, each in columns of up to 128 bytes a key (what a TMA box with the swizzle of
 // that width leaves): the 16-byte pieces of a column's row are rotated by the row, so that eight rows' equal pieces lie in
 // eight bank groups.
@@ -359,6 +370,51 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const __grid_consta
                     limbs(x, y, l);
 #pragma unroll
                     for (int i = 0; i < L; ++i) wf[nq][o][i] = transposed(l[i]);
+                }
+            }
+            if (edge) {   // a weight of 0 times a value that is not finite must be 0: such values are taken out and added where they are seen
+                unsigned keys = 0;
+#pragma unroll 1
+                for (int e = lane; e < STEP * St::PIECES; e += 32) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(st + St::POOL + St::at(e / St::PIECES, e % St::PIECES));
+                    if (not_finite<F32S>(x.x) || not_finite<F32S>(x.y) || not_finite<F32S>(x.z) || not_finite<F32S>(x.w)) keys |= 1u << (e / St::PIECES);
+                }
+                keys = __reduce_or_sync(0xffffffffu, keys);
+                if (keys) {
+#pragma unroll 1
+                    for (unsigned left = keys; left; left &= left - 1) {
+                        const int key = __ffs(left) - 1;
+#pragma unroll
+                        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const float x = __shfl_sync(0xffffffffu, key < 8 ? s[nq][half] : s[nq][2 + half], (key & 7) * 4 + tq);
+#pragma unroll
+                                for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                                    for (int o = 0; o < 2; ++o) {
+                                        const int ch = 16 * mb + 8 * o + g;
+                                        const unsigned char* at = st + St::POOL + St::at(key, ch * (int)sizeof(TS) / 16) + ch * (int)sizeof(TS) % 16;
+                                        float v;
+                                        if constexpr (F32S) v = *reinterpret_cast<const float*>(at);
+                                        else v = bf16_to_f(*reinterpret_cast<const uint16_t*>(at));
+                                        if (x > -INFINITY && !(fabsf(v) < INFINITY)) acc[nq][mb][2 * o + half] += v;
+                                    }
+                            }
+                    }
+                    __syncwarp();
+#pragma unroll 1
+                    for (int e = lane; e < STEP * St::PIECES; e += 32) {
+                        uint4* at = reinterpret_cast<uint4*>(st + St::POOL + St::at(e / St::PIECES, e % St::PIECES));
+                        uint4 x = *at;
+                        x.x = finite_only<F32S>(x.x);
+                        x.y = finite_only<F32S>(x.y);
+                        x.z = finite_only<F32S>(x.z);
+                        x.w = finite_only<F32S>(x.w);
+                        *at = x;
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next copy into this stage comes after
+                    __syncwarp();
                 }
             }
 #pragma unroll

@@ -9,9 +9,11 @@
 // units.  Two groups of 128 threads work on half a tile each: while one turns its scores into weights the tensor cores
 // multiply for the other.
 // Keys and values come by TMA, a box per page and 64 channels, into rings of their own; a page outside the store, or past
-// the stretch, is a coordinate past the tensor's last page, which TMA fills with zeros without reading.  Rows of V in
-// front of the stretch or behind it (the rest of a page, left padding) are written over with zeros in shared memory before
-// the multiply: a weight of 0 times whatever lies there must be 0.
+// the stretch, is a coordinate past the tensor's last page, which TMA fills with zeros without reading.
+// A weight of 0 times whatever lies in a hidden place must be 0.  So a warp goes over the units that some row sees only in
+// part before they are multiplied: rows of V in front of the stretch or behind it (the rest of a page, left padding) become
+// zeros, and so do values that are not finite (a later token's, which earlier rows do not see); the rows that do see
+// those get them added behind the multiplies.
 // With f32 queries Q and P are three bf16 limbs each (L 3): three products per step instead of one.
 //
 // P is written over its S.  Each group has two such places, so the scores of the
@@ -36,7 +38,7 @@ namespace {
 
 using namespace tcc;
 
-constexpr int THREADS = 384;             // two groups of 128 rows, a warp per group that issues multiplies, the copies' warp
+constexpr int THREADS = 384;             // two groups of 128 rows, a warp per group that issues multiplies, the copies' warp, the sweeping one
 constexpr uint32_t PLACES = 2;           // of scores and weights, per group
 struct Plan {                            // of the line: a tile's queries and results take as long as four units
     static constexpr int MR = 256, KT = 64, START = 4, SNAP = 4;
@@ -44,14 +46,25 @@ struct Plan {                            // of the line: a tile's queries and re
 constexpr int MR = Plan::MR, KT = Plan::KT;
 constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by before the sums are rescaled
 
+// Units of a run in which values that are not finite were taken out of V: their keys.  A run can have at most so many units
+// that some row sees in part (the diagonal's and a window's other end); the sweeping warp is at most as many runs ahead of
+// the rows as the ring has units.
+struct Found {
+    int count;
+    int unit[15];
+    uint64_t keys[15];
+};
+constexpr uint32_t RUNS = 16;
+
 template <int HS_, int L_>
 struct Shape {
     static constexpr int HS = HS_, L = L_;
     static constexpr int HALVES = HS / 64;                           // 64-channel columns of 128 bytes a row
     static constexpr uint32_t Q_LIMB = 128 * HS * 2, Q_TILE = L * Q_LIMB, KV = KT * HS * 2;
-    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 8) : 5;   // units in shared memory
+    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 7) : 4;   // units in shared memory
     static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_V = OFF_K + RING * KV, OFF_BAR = OFF_V + RING * KV;
-    static constexpr uint32_t BYTES = OFF_BAR + 768 + 1024;          // the rest: alignment to 1024
+    static constexpr uint32_t OFF_FOUND = OFF_BAR + 768;             // Found[RUNS]
+    static constexpr uint32_t BYTES = OFF_FOUND + RUNS * sizeof(Found) + 1024;   // the rest: alignment to 1024
     // Tensor memory of a group: places of scores and weights, the mix.  A place's scores are read a chunk at a time and the
     // weights go back over it: the first limb in its first half, the second in the second, the third outside.
     static __device__ __forceinline__ uint32_t weights_at(int l, int c) { return l == 2 ? 64 + c / 2 : c + CW / 2 * l; }   // of the chunk of keys from c on
@@ -239,6 +252,9 @@ struct Run {
     int ta, tb, rows;
     int a[2], b[2];
     __device__ __forceinline__ int count(int w) const { return max(b[w] - a[w], 0); }
+    int all_from, all_to;                // keys that every row of the tile sees
+    // whether the sweeping warp goes over unit t: some row does not see all of it
+    __device__ __forceinline__ bool swept(int t) const { return t * KT < all_from || t * KT + KT > all_to; }
 };
 __device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, long long u, long long end) {
     Run r;
@@ -249,6 +265,8 @@ __device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, 
     r.ta = none ? 0 : it.s.lo / KT + s.from;
     r.tb = none ? 0 : it.s.lo / KT + s.to;
     r.rows = min(it.q.f * a.group - it.tile * MR, MR);
+    r.all_to = it.q.c + it.tile * MR / a.group + 1;
+    r.all_from = a.window > 0 ? max(it.q.first, it.q.c + (it.tile * MR + r.rows - 1) / a.group + 1 - a.window) : it.q.first;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         r.a[w] = r.b[w] = r.ta;
@@ -262,6 +280,31 @@ __device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, 
         }
     }
     return r;
+}
+
+// Adds what the sweeping warp has taken out of V to a row that sees it, in its results or in its end (the thread's own
+// writes): an infinity or a NaN is what its mix then is.
+template <int HS>
+__device__ __noinline__ void add_found(const ReadArgs& a, const split::Item& it, const volatile Found* found, int low, int pos, int from, int to, float* end, int64_t out_at) {
+    const int32_t* pages = a.table + (int64_t)it.r * a.max_pages;
+    for (int f = 0; f < found->count; ++f) {
+        const int t = found->unit[f];
+        if (t < from || t >= to) continue;
+        for (uint64_t keys = found->keys[f]; keys; keys &= keys - 1) {
+            const int j = t * KT + __ffsll((long long)keys) - 1;
+            if (j < low || j > pos) continue;
+            const int page = pages[j / a.s.page_size];
+            if (page < 0 || page >= a.s.n_pages) continue;
+            const uint16_t* v = static_cast<const uint16_t*>(a.s.v) + page * a.s.page_stride + it.head * a.s.head_stride + (j % a.s.page_size) * a.s.place_stride;
+            for (int c = 0; c < HS; ++c) {
+                if ((v[c] & 0x7f80u) != 0x7f80u) continue;
+                const float x = bf16_to_f(v[c]);
+                if (end) end[c] += x;
+                else if (a.bf16_q) static_cast<uint16_t*>(a.out)[out_at + c] = f_to_bf16(bf16_to_f(static_cast<uint16_t*>(a.out)[out_at + c]) + x);
+                else static_cast<float*>(a.out)[out_at + c] += x;
+            }
+        }
+    }
 }
 
 template <typename Sh>
@@ -290,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         cuts[worker].workers = 0;
         for (uint32_t i = 0; i < RING; ++i) {
             bar_init(&bars->full[i], 1);
-            bar_init(&bars->empty[i], 2);     // each group has used it or passed it over
+            bar_init(&bars->empty[i], 3);     // each group has used it or passed it over, the sweeping warp has been there
             bar_init(&bars->passed[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
@@ -324,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         const uint32_t mine = tmem + w * Sh::GROUP + ((uint32_t)((warp & 3) * 32) << 16);
         const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;   // its sign is in the queries
         const bool out_wide = !((reinterpret_cast<uintptr_t>(a.out) & 15) || (a.out_token_stride % (L == 3 ? 4 : 8)) || (a.out_head_stride % (L == 3 ? 4 : 8)));
-        uint32_t n_p = 0;                // units of this group so far: its barriers' phases
+        uint32_t n_p = 0, runs = 0;      // units of this group so far: its barriers' phases; runs with units
         // A run's queries, a row per thread, into the operand layout.  They are brought as soon as the scores of the run
         // before are made, in front of its epilogue, so that the first scores of the next run are ready behind it.
         constexpr int CH = L == 3 ? 4 : 8;   // channels in 16 bytes
@@ -578,13 +621,22 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     cuts[worker].workers = (int)split::last_worker<Plan>(it, per) - worker + 1;
                 }
             }
+            if (units > 0 && live && (run.swept(run.a[w]) || run.swept(run.b[w] - 1))) {
+                const volatile Found* found = reinterpret_cast<const Found*>(smem + Sh::OFF_FOUND) + runs % RUNS;
+                if (found->count > 0) {          // values that are not finite have been taken out: the row gets those that it sees
+                    float* row_end = ends + ((int64_t)worker * 2 + (u == it.begin ? 1 : 0)) * Ends<HS, MR>::FLOATS + q_row * HS;
+                    add_found<HS>(a, it, found, low, pos, run.a[w], run.b[w], whole ? nullptr : row_end,
+                                  (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride);
+                }
+            }
+            if (run.ta < run.tb) ++runs;
             tc_before();
             if (units > 0) warp_arrive(&bars->o_free[w]);
             u = run.stop;
             if (u < end) split::next<Plan>(a, it);
         }
     } else if (warp < 10) {
-        // ---- a group's multiplies: one lane issues, the warp clears the rows of V that belong to nobody
+        // ---- a group's multiplies: one lane issues
         constexpr uint32_t i_s = instr_desc(KT), i_o = instr_desc(HS) | (1u << 16);   // V with its keys down
         const int w = warp - 8;
         const uint32_t d = tmem + w * Sh::GROUP;
@@ -601,7 +653,6 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 if (ok && lane == 0) {
                     const uint32_t slot = (base + (uint32_t)(t - run.ta)) % RING;
                     bar_arrive(&bars->empty[slot]);
-                    if (w == 0) bar_arrive(&bars->passed[slot]);
                 }
             };
             auto scores = [&](int t) {           // of unit t, which has landed, into the next place
@@ -637,21 +688,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             for (int t = from; t < to && ok; ++t) {
                 const uint32_t seq = base + (uint32_t)(t - run.ta), slot = seq % RING, place = n_p % PLACES;
                 const bool first = t == from, fresh_sum = FLUSH ? (t - from) % (FLUSH ? FLUSH : 1) == 0 : first;
-                const int clear_to = it.s.lo - t * KT, clear_from = it.s.hi - t * KT;   // rows in front of the stretch, and behind it
-                if (clear_to > 0 || clear_from < KT) {
-                    unsigned char* v = smem + Sh::OFF_V + slot * Sh::KV;
-                    if (w == 1 && t >= run.a[0] && t < run.b[0]) {   // the first group clears what both use
-                        ok = warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
-                    } else {
-                        for (int e = lane; e < KT * (HS / 8); e += 32) {
-                            const int key = e / (HS / 8), c = e % (HS / 8);
-                            if (key < clear_to || key >= clear_from) *reinterpret_cast<uint4*>(v + (c / 8) * (KT * 128) + swz128(key, (c & 7) * 8)) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_async();
-                    }
-                    __syncwarp();
-                }
-                if (w == 0 && lane == 0) bar_arrive(&bars->passed[slot]);
+                if (run.swept(t)) ok = ok && warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
                 if (t + (int)PLACES < to) full(t + PLACES);          // waited for before the weights are: nothing but the mix and
                 if (first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);   // its completion lies
                 ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);              // between them and the next scores
@@ -721,6 +758,62 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
         if (!ok) {   // the copies in flight end before the block does
             for (uint32_t back = 1; back <= RING && back <= n; ++back) bar_wait(&bars->full[(n - back) % RING], ((n - back) / RING) & 1);
+        }
+    } else {
+        // ---- the sweeping warp
+        uint32_t n = 0, runs = 0;
+        while (u < end && ok) {
+            const Run run = run_of(a, it, u, end);
+            volatile Found* found = reinterpret_cast<Found*>(smem + Sh::OFF_FOUND) + runs % RUNS;
+            int count = 0;
+            for (int t = run.ta; t < run.tb && ok; ++t, ++n) {
+                const uint32_t slot = n % RING;
+                ok = warp_wait(&bars->full[slot], (n / RING) & 1, failed);
+                if (!ok) break;
+                if (run.swept(t)) {
+                    unsigned char* v = smem + Sh::OFF_V + slot * Sh::KV;
+                    const int clear_to = it.s.lo - t * KT, clear_from = it.s.hi - t * KT;   // rows in front of the stretch, and behind it
+                    uint64_t keys = 0;
+                    for (int e = lane; e < KT * (HS / 8); e += 32) {
+                        const int key = e / (HS / 8), c = e % (HS / 8);
+                        uint4* at = reinterpret_cast<uint4*>(v + (c / 8) * (KT * 128) + swz128(key, (c & 7) * 8));
+                        if (key < clear_to || key >= clear_from) {
+                            *at = make_uint4(0, 0, 0, 0);
+                            continue;
+                        }
+                        uint4 x = *at;
+                        uint32_t* y = reinterpret_cast<uint32_t*>(&x);
+                        bool any = false;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {   // an exponent of all ones, in either half
+                            const uint32_t m = ((y[k] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((y[k] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+                            any |= m != 0;
+                            y[k] &= ~m;
+                        }
+                        if (any) {
+                            *at = x;
+                            keys |= 1ull << key;
+                        }
+                    }
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) keys |= __shfl_xor_sync(0xffffffffu, keys, o);
+                    if (keys && count < 15) {
+                        if (lane == 0) {
+                            found->unit[count] = t;
+                            found->keys[count] = keys;
+                        }
+                        ++count;
+                    }
+                    fence_async();
+                }
+                __threadfence_block();
+                if (lane == 0) found->count = count;
+                warp_arrive(&bars->passed[slot]);
+                if (lane == 0) bar_arrive(&bars->empty[slot]);
+            }
+            if (run.ta < run.tb) ++runs;
+            u = run.stop;
+            if (u < end) split::next<Plan>(a, it);
         }
     }
     if (!ok && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_WAIT_RAN_OUT);

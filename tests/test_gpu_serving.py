@@ -472,6 +472,38 @@ def test_attend_infinite_and_nan_keys_that_are_hidden_do_not_leak(T, S, dt, fres
     check_attend(T, x, out, lse, 0.125)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("hs", [32, 64, 128])
+@pytest.mark.parametrize("fresh,page,window", [(2, 16, 0), (5, 24, 0), (9, 16, 6), (40, 8, 0), (200, 16, 0), (300, 64, 100), (130, 100, 0)])
+def test_attend_values_that_are_not_finite_reach_the_rows_that_see_them_only(T, S, dt, hs, fresh, page, window):
+    """Infinite and NaN values of single new tokens, of one stored one, and of one in front of the padding: a row that
+    sees none of them is the finite row; one that sees them is not finite in that channel, and finite elsewhere."""
+    rng = np.random.default_rng(fresh + hs)
+    first = [0, 30, 0]
+    x = attend_inputs(T, rng, [(70, fresh), (64, fresh), (3, 1)], 4, 2, hs, page, dt, first=first)
+    clean = call_attend(T, S, x, 0.125, window)
+    check_attend(T, x, *clean, 0.125, window)
+    marks = [(0, 70 + fresh - 1, 3, float("nan")), (0, 70 + fresh // 2, 5, float("inf")), (0, 20, 7, -float("inf")), (1, 64 + fresh // 3, hs - 1, float("inf")),
+             (1, 29, 9, float("nan"))]
+    for r, j, ch, v in marks:
+        x["vp"][int(x["table"][r, j // page]), 1, j % page, ch] = v
+    out, lse = call_attend(T, S, x, 0.125, window)
+    assert T.equal(lse, clean[1])
+    at = 0
+    for r, (c, f) in enumerate(x["lengths"]):
+        pos = T.arange(c, c + f, device="cuda:0")
+        bad = T.zeros(f, hs, dtype=T.bool, device="cuda:0")
+        for rr, j, ch, v in marks:
+            if rr == r and j >= first[r]:
+                bad[:, ch] |= (pos >= j) & ((pos - j < window) if window else (pos >= 0))
+        o, o0 = out[at:at + f].float(), clean[0][at:at + f].float()
+        assert T.equal(o[:, :2], o0[:, :2]), r                       # the other key head
+        assert T.isfinite(o[:, 2:][~bad[:, None].expand(-1, 2, -1)]).all(), r
+        assert not T.isfinite(o[:, 2:][bad[:, None].expand(-1, 2, -1)]).any(), r
+        assert T.equal(o[:, 2:][~bad[:, None].expand(-1, 2, -1)], o0[:, 2:][~bad[:, None].expand(-1, 2, -1)]), r
+        at += f
+
+
 def test_attend_takes_offsets_beyond_32_bits(T, S):
     """Pages that lie more than 2^31 elements into the pools (k and v share one)."""
     rng = np.random.default_rng(6)
