@@ -282,6 +282,8 @@ __device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, 
     return r;
 }
 
+__device__ __forceinline__ void next_item(const ReadArgs& a, split::Item& it) { split::next<Plan>(a, it); }
+
 // Adds what the sweeping warp has taken out of V to a row that sees it, in its results or in its end (the thread's own
 // writes): an infinity or a NaN is what its mix then is.
 template <int HS>
@@ -418,12 +420,6 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             fence_async();
             warp_arrive(&bars->q_ready[w]);
         };
-        auto bring_next = [&](long long stop) {
-            if (stop >= end) return;
-            split::Item then = it;
-            split::next<Plan>(a, then);
-            bring(then, run_of(a, then, stop, end));
-        };
         if (u < end) bring(it, run_of(a, it, u, end));
         while (u < end && ok) {
             const Run run = run_of(a, it, u, end);
@@ -436,18 +432,6 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             uint64_t acc[FLUSH ? HS / 2 : 1];    // the mix of the units that have been flushed
 #pragma unroll
             for (int k = 0; k < (FLUSH ? HS / 2 : 1); ++k) acc[k] = 0ull;
-            auto flush = [&]() {                 // the units before this one have been added up in tensor memory: their sum joins acc
-                ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
-                tc_after();
-#pragma unroll
-                for (int c = 0; c < (FLUSH ? HS : 0); c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(mine + Sh::C_O + c, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) acc[c / 2 + k] = add2(acc[c / 2 + k], two(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])));
-                }
-            };
             for (int n = 0; n < units && ok; ++n) {
                 const int t = run.a[w] + n;
                 const uint32_t place = n_p % PLACES, at = mine + place * Sh::PLACE;
@@ -474,17 +458,28 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 }
                 const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
                 const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
-                bool due = FLUSH && n > 0 && n % (FLUSH ? FLUSH : 1) == 0;
-                if (__any_sync(0xffffffffu, grown)) {
+                const bool due = FLUSH && n > 0 && n % (FLUSH ? FLUSH : 1) == 0;
+                const bool some = __any_sync(0xffffffffu, grown);
+                if (n > 0 && (due || some)) {    // once the unit before has been added up
+                    ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
+                    if (!ok) break;
+                    tc_after();
+                }
+                if constexpr (FLUSH > 0) {
+                    if (due) {                   // the mix so far joins acc; the next one starts anew
+#pragma unroll
+                        for (int c = 0; c < HS; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(mine + Sh::C_O + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) acc[c / 2 + k] = add2(acc[c / 2 + k], two(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])));
+                        }
+                    }
+                }
+                if (some) {
                     const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
-                    if (due) {
-                        flush();
-                        if (!ok) break;
-                        due = false;
-                    } else if (n > 0) {   // once the unit before has been added up
-                        ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
-                        if (!ok) break;
-                        tc_after();
+                    if (n > 0 && !due) {
 #pragma unroll 1
                         for (int c = 0; c < HS; c += 32) {
                             uint32_t o[32];
@@ -537,15 +532,16 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 apart(add2(part[0], part[1]), x, y);
                 sum += x + y;
                 tmem_wait_st();
-                if (due) {
-                    flush();
-                    if (!ok) break;
-                }
                 tc_before();
                 warp_arrive(&bars->p_ready[w][place]);
                 ++n_p;
             }
-            if (ok) bring_next(run.stop);   // every score of this run has been made
+            if (!ok) break;
+            if (run.stop < end) {
+                split::Item then = it;
+                next_item(a, then);
+                bring(then, run_of(a, then, run.stop, end));
+            }
             // ---- the read of the row, or this piece's end of it
             if (units > 0 && ok) ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
             if (!ok) break;
@@ -582,8 +578,12 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
 #pragma unroll
                         for (int k = 0; k < 32; k += 4) {
                             if (out_wide) *reinterpret_cast<float4*>(out + k) = make_float4(x[k] * inv, x[k + 1] * inv, x[k + 2] * inv, x[k + 3] * inv);
-                            else
-                                for (int y = 0; y < 4; ++y) out[k + y] = x[k + y] * inv;
+                            else {
+                                out[k] = x[k] * inv;
+                                out[k + 1] = x[k + 1] * inv;
+                                out[k + 2] = x[k + 2] * inv;
+                                out[k + 3] = x[k + 3] * inv;
+                            }
                         }
                     } else {
                         uint16_t* out = static_cast<uint16_t*>(a.out) + to + c;
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             tc_before();
             if (units > 0) warp_arrive(&bars->o_free[w]);
             u = run.stop;
-            if (u < end) split::next<Plan>(a, it);
+            if (u < end) next_item(a, it);
         }
     } else if (warp < 10) {
         // ---- a group's multiplies: one lane issues
@@ -655,9 +655,39 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     bar_arrive(&bars->empty[slot]);
                 }
             };
-            auto scores = [&](int t) {           // of unit t, which has landed, into the next place
-                const uint32_t slot = (base + (uint32_t)(t - run.ta)) % RING, place = n_s % PLACES;
-                if (!ok) return;
+            for (int t = run.ta; t < min(from, run.tb) && ok; ++t) pass(t);
+            if (from < to) ok = ok && warp_wait(&bars->q_ready[w], n_run & 1, failed);
+            // a step: the mix of unit t, and as soon as that is done the scores of the unit that takes its place
+#pragma unroll 1
+            for (int t = from - (int)PLACES; t < to && ok; ++t) {
+                const int ts = t + (int)PLACES;
+                if (ts < to) full(ts);           // waited for before the weights are: nothing but the mix lies between them and the next scores
+                if (t >= from) {
+                    const uint32_t seq = base + (uint32_t)(t - run.ta), slot = seq % RING, place = n_p % PLACES;
+                    const bool first = t == from, fresh_sum = FLUSH ? (t - from) % (FLUSH ? FLUSH : 1) == 0 : first;
+                    if (run.swept(t)) ok = ok && warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
+                    if (first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);
+                    ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);
+                    if (!ok) break;
+                    if (elected()) {
+                        tc_after();
+                        const uint32_t at_v = at0 + Sh::OFF_V + slot * Sh::KV;
+#pragma unroll
+                        for (int l = L - 1; l >= 0; --l)
+#pragma unroll
+                            for (int c = 0; c < KT / 16; ++c)
+                                mma_ts(d + Sh::C_O, d + place * Sh::PLACE + Sh::weights_at(l, 16 * c / CW * CW) + 16 * c % CW / 2, desc_keys_down(at_v + c * 2048, KT * 128),
+                                       i_o, !fresh_sum || l < L - 1 || c > 0);
+                        commit(&bars->pv_done[w][place]);
+                        commit(&bars->empty[slot]);
+                    }
+                    __syncwarp();
+                    ++n_p;
+                }
+                if (ts >= to) continue;
+                const uint32_t place = n_s % PLACES, slot = (base + (uint32_t)(ts - run.ta)) % RING;
+                if (n_s >= PLACES) ok = ok && warp_wait(&bars->pv_done[w][place], ((n_s - PLACES) / PLACES) & 1, failed);
+                if (!ok) break;
                 if (elected()) {
                     tc_after();
                     const unsigned char* q = smem + w * Sh::Q_TILE;
@@ -672,51 +702,12 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 }
                 __syncwarp();
                 ++n_s;
-            };
-            for (int t = run.ta; t < min(from, run.tb) && ok; ++t) pass(t);
-            if (from < to) {
-                ok = ok && warp_wait(&bars->q_ready[w], n_run & 1, failed);
-                // the first two units' scores: what their places held before has been mixed
-#pragma unroll 1
-                for (int t = from; t < min(to, from + (int)PLACES) && ok; ++t) {
-                    full(t);
-                    if (n_s >= PLACES) ok = ok && warp_wait(&bars->pv_done[w][n_s % PLACES], ((n_s - PLACES) / PLACES) & 1, failed);
-                    scores(t);
-                }
-            }
-#pragma unroll 1
-            for (int t = from; t < to && ok; ++t) {
-                const uint32_t seq = base + (uint32_t)(t - run.ta), slot = seq % RING, place = n_p % PLACES;
-                const bool first = t == from, fresh_sum = FLUSH ? (t - from) % (FLUSH ? FLUSH : 1) == 0 : first;
-                if (run.swept(t)) ok = ok && warp_wait(&bars->passed[slot], (seq / RING) & 1, failed);
-                if (t + (int)PLACES < to) full(t + PLACES);          // waited for before the weights are: nothing but the mix and
-                if (first && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);   // its completion lies
-                ok = ok && warp_wait(&bars->p_ready[w][place], (n_p / PLACES) & 1, failed);              // between them and the next scores
-                if (!ok) break;
-                if (elected()) {
-                    tc_after();
-                    const uint32_t at_v = at0 + Sh::OFF_V + slot * Sh::KV;
-#pragma unroll
-                    for (int l = L - 1; l >= 0; --l)
-#pragma unroll
-                        for (int c = 0; c < KT / 16; ++c)
-                            mma_ts(d + Sh::C_O, d + place * Sh::PLACE + Sh::weights_at(l, 16 * c / CW * CW) + 16 * c % CW / 2, desc_keys_down(at_v + c * 2048, KT * 128), i_o,
-                                   !fresh_sum || l < L - 1 || c > 0);
-                    commit(&bars->pv_done[w][place]);
-                    commit(&bars->empty[slot]);
-                }
-                __syncwarp();
-                if (t + (int)PLACES < to) {
-                    ok = warp_wait(&bars->pv_done[w][place], (n_p / PLACES) & 1, failed);
-                    scores(t + PLACES);
-                }
-                ++n_p;
             }
             for (int t = max(to, run.ta); t < run.tb && ok; ++t) pass(t);
             if (from < to) ++n_run;
             base += (uint32_t)(run.tb - run.ta);
             u = run.stop;
-            if (u < end) split::next<Plan>(a, it);
+            if (u < end) next_item(a, it);
         }
     } else if (warp == 10) {
         // ---- the copies: a lane per box
@@ -753,7 +744,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 __syncwarp();
             }
             u = run.stop;
-            if (u < end) split::next<Plan>(a, it);
+            if (u < end) next_item(a, it);
         }
         if (__any_sync(0xffffffffu, bad_page) && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_BAD_PAGE);
         if (!ok) {   // the copies in flight end before the block does
@@ -813,7 +804,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             }
             if (run.ta < run.tb) ++runs;
             u = run.stop;
-            if (u < end) split::next<Plan>(a, it);
+            if (u < end) next_item(a, it);
         }
     }
     if (!ok && lane == 0 && a.status) atomicOr(a.status, AVA_PAGED_WAIT_RAN_OUT);
