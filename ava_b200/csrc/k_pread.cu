@@ -145,8 +145,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const __grid_consta
     const int w = blockIdx.x * WARPS + warp;
     const long long per = max((line.total() + workers - 1) / workers, 1ll);
     split::Item it = {}, after = {};
+    it.r = -1;
     long long u = split::piece<Pl>(a, line, per, w, &it);
-    const long long end = split::piece<Pl>(a, line, per, w + 1ll, &after);
+    const long long end = split::piece<Pl>(a, line, per, w + 1ll, &after, &it);
     if (lane == 0) cuts[w].workers = 0;
     unsigned char* ring = smem + warp * STAGES * St::BYTES;
     uint64_t* bar = bars + warp * STAGES;

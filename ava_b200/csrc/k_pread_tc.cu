@@ -329,8 +329,9 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
     const int worker = blockIdx.x;
     const long long per = max((line.total() + gridDim.x - 1) / (long long)gridDim.x, 1ll);
     split::Item it = {}, after = {};
+    it.r = -1;
     long long u = split::piece<Plan>(a, line, per, worker, &it);
-    const long long end = split::piece<Plan>(a, line, per, worker + 1ll, &after);
+    const long long end = split::piece<Plan>(a, line, per, worker + 1ll, &after, &it);
     if (tid == 0) {
         cuts[worker].workers = 0;
         for (uint32_t i = 0; i < RING; ++i) {
@@ -846,7 +847,11 @@ cudaError_t launch_one(int device, cudaStream_t st, const ReadArgs& a, void* roo
 cudaError_t launch_paged_read_tc(int device, cudaStream_t st, const ReadArgs& a, void* room, int sms, bool* taken) {
     *taken = false;
     PoolShape pool;
-    if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && !(a.s.head_size == 128 && a.bf16_q)) || (int64_t)a.max_fresh * a.group <= (a.bf16_q ? 32 : 64) || !pool_shape(a.s, &pool))
+    // Few rows per key head stay with the warp kernel, whose tiles of 8 to 32 rows read the store once.  Measured at 32 requests
+    // of 4096 keys, 8 key heads (warp kernel / this one): 24 rows 91 / 115 us and 32 rows 140 / 114 us at 128 channels, 32
+    // rows 86 / 101 us and 48 rows 118 / 101 us at 64; f32 queries 24 rows 101 / 150 us, 48 rows 197 / 154 us.
+    const int64_t few = a.s.head_size == 128 ? 24 : 32;
+    if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && !(a.s.head_size == 128 && a.bf16_q)) || (int64_t)a.max_fresh * a.group <= few || !pool_shape(a.s, &pool))
         return cudaSuccess;
     if (a.s.head_size == 64) return a.bf16_q ? launch_one<64, 1>(device, st, a, room, sms, pool, taken) : launch_one<64, 3>(device, st, a, room, sms, pool, taken);
     return launch_one<128, 1>(device, st, a, room, sms, pool, taken);

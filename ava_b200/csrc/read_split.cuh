@@ -133,22 +133,24 @@ struct Item {
     long long begin;            // where the stretch's START units begin; its own follow
 };
 
-// The stretch that place u of the line lies in (u < total), by a warp together.
+// The stretch that place u of the line lies in (u < total), by a warp together.  known (may be null): an item whose request
+// need not be looked at again.
 template <typename P>
-__device__ __forceinline__ Item locate(const ReadArgs& a, const Line& l, long long u) {
+__device__ __forceinline__ Item locate(const ReadArgs& a, const Line& l, long long u, const Item* known) {
     int lo = 0, hi = l.entries;
     while (hi - lo > 1) {       // the last entry whose sum is not above u: empty requests are passed over
         const int mid = (lo + hi) >> 1;
         if (l.sums[mid] <= u) lo = mid;
         else hi = mid;
     }
-    Item it;
+    Item it = {};
     bool bad = false;
     it.begin = l.sums[lo];
     it.r = lo * l.step;
     long long n = 0;
     for (;; ++it.r) {
-        it.q = request(a, it.r, &bad);
+        if (known && known->r == it.r) it.q = known->q;
+        else it.q = request(a, it.r, &bad);
         n = l.step == 1 ? l.sums[lo + 1] - it.begin : head_units_warp<P>(a, it.q) * a.s.kv_heads;
         if (u < it.begin + n) break;
         it.begin += n;
@@ -198,10 +200,10 @@ __device__ __forceinline__ void next(const ReadArgs& a, Item& it) {
 // Where worker w's piece begins; a place inside a stretch of at most SNAP units, or within START + SNAP / 2 units of a
 // stretch's beginning, moves to that beginning.
 template <typename P>
-__device__ __forceinline__ long long piece(const ReadArgs& a, const Line& l, long long per, long long w, Item* it) {
+__device__ __forceinline__ long long piece(const ReadArgs& a, const Line& l, long long per, long long w, Item* it, const Item* known = nullptr) {
     const long long u = w * per;
     if (u >= l.total()) return l.total();
-    *it = locate<P>(a, l, u);
+    *it = locate<P>(a, l, u, known);
     return it->s.units <= P::SNAP || u <= it->begin + P::START + P::SNAP / 2 ? it->begin : u;
 }
 
