@@ -226,12 +226,12 @@ __global__ void __launch_bounds__(V_THREADS, 4) verify_kernel(const VerifyArgs a
         mine = -1;
         for (int k = 0; k < parts && !found; ++k) {
             const double s = totals[attempt][k];
-            if (s > 0.0) {
+            if (s > 0.0) {          // a part without mass is never it, whatever the number drawn (below 0 too)
                 mine = k;
                 before = run;
+                run += s;
+                found = run > target;
             }
-            run += s;
-            found = run > target;
         }
         if ((whole > 0.0 && whole < INFINITY) || (!w.q && w.without < 0)) break;
         w.q = nullptr;    // no mass in the difference: the target's own

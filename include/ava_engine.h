@@ -575,7 +575,8 @@ int ava_paged_attend(int device, void* stream, const ava_paged_store* store, con
  *   the token behind the accepted ones is drawn from max(p - q, 0) of the refused draft's row (q NULL: p without the draft;
  *   all accepted: p of the last row): the lowest token whose running sum, in token order, exceeds
  *   uniform[q_start[r] + n] * the whole sum
- * so that the tokens are distributed as the target's own.  Products and sums in f64; a probability that is negative or NaN
+ * so that the tokens are distributed as the target's own.  uniform lies in [0, 1) (below: as 0; else, NaN among it: as the
+ * largest below 1, the last token with any mass).  Products and sums in f64; a probability that is negative or NaN
  * counts as 0; a difference without mass falls back to p, p without mass gives AVA_NO_TOKEN and NO_MASS.  uniform NULL:
  * greedy, p may be logits; a draft is accepted while it is its row's largest value (lowest token among equals, NaN never),
  * and the token behind is the largest of its row.

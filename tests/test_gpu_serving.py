@@ -682,6 +682,16 @@ def test_verify_flags_what_it_cannot_use(T, S):
     assert out[0].tolist() == [0, 0] and status == 0
 
 
+@pytest.mark.parametrize("vocab", [64, 40000])
+def test_verify_numbers_outside_their_range_still_draw_a_token_with_mass(T, S, vocab):
+    p = np.zeros((1, vocab), np.float32)
+    p[0, [vocab // 2, vocab - 3]] = 0.5
+    for u, want in ((-0.5, vocab // 2), (-np.inf, vocab // 2), (1.0, vocab - 3), (7.0, vocab - 3), (np.inf, vocab - 3), (np.nan, vocab - 3)):
+        for rows in (1, 700):
+            out, n, status = call_verify(T, S, np.repeat(p, rows, 0), None, np.zeros(rows), np.arange(rows + 1), np.full(rows, u), 2)
+            assert (out == [want, -1]).all() and n == [1] * rows and status == 0, (u, rows)
+
+
 def test_verify_keeps_the_targets_distribution(T, S):
     """Many independent draws of one draft each: the first token's frequencies are p's, whatever q is."""
     rng = np.random.default_rng(1)
