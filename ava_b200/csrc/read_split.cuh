@@ -17,6 +17,7 @@
 namespace ava {
 namespace split {
 
+constexpr long long MOST_KEYS = 1ll << 29;   // of a request: a warp's tiles together stay within 32 bits of units
 constexpr int ENTRIES = 2048;   // sums over requests kept in shared memory (each of several requests when there are more)
 
 struct Request {
@@ -32,7 +33,7 @@ __device__ __forceinline__ Request request(const ReadArgs& a, int r, bool* bad) 
     q.first = a.first ? max(a.first[r], 0) : 0;
     q.f = end - q.start;
     const long long total = (long long)q.c + q.f;
-    if (q.start < 0 || end < q.start || end > a.max_tokens || q.c < 0 || total > (long long)a.max_pages * a.s.page_size || total > 0x7ffffff0ll) {
+    if (q.start < 0 || end < q.start || end > a.max_tokens || q.c < 0 || total > (long long)a.max_pages * a.s.page_size || total >= MOST_KEYS) {
         q.f = 0;
         *bad = true;
     }

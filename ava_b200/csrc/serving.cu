@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cstdint>
 #include <string>
+#include <utility>
 
 #include "../../include/ava_engine.h"
 #include "serving.cuh"
@@ -69,12 +70,34 @@ int sm_count(int device) {
     return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess ? n : 0;
 }
 
+// Indexes of requests, tokens and pages are 32 bits in the kernels, with room for a block's stride behind the last.
+constexpr int32_t MOST_ROWS = 1 << 24, MOST_TOKENS = 1 << 30, MOST_PAGES = 1 << 30;
+
+// Whether an array that is written has no element twice: extents and strides of its dimensions but the innermost, which
+// holds `inner` adjacent elements.  Sorted by stride each must reach over all inside it (a broadcast has stride 0).
+template <int N>
+bool distinct(int64_t inner, int64_t (&n)[N], int64_t (&stride)[N]) {
+    for (int i = 1; i < N; ++i)
+        for (int j = i; j > 0 && stride[j] < stride[j - 1]; --j) {
+            std::swap(stride[j], stride[j - 1]);
+            std::swap(n[j], n[j - 1]);
+        }
+    __int128 reach = inner;
+    for (int i = 0; i < N; ++i) {
+        if (n[i] <= 1) continue;
+        if (stride[i] < reach) return false;
+        reach += static_cast<__int128>(n[i] - 1) * stride[i];
+    }
+    return true;
+}
+
 // What append and attend need of a store; nullptr: fine.
 const char* store_fault(const ava_paged_store* s) {
     if (!s || !s->k || !s->v) return "a store without its pools";
     if (s->dtype != AVA_F32 && s->dtype != AVA_BF16) return "the store's dtype is AVA_F32 or AVA_BF16";
     if (s->n_pages <= 0 || s->kv_heads <= 0 || s->page_size <= 0 || s->head_size <= 0) return "the store's sizes must be positive";
     if (s->page_stride < 0 || s->head_stride < 0 || s->place_stride < s->head_size) return "the store's strides: not negative, places at least a head apart";
+    if (static_cast<int64_t>(s->kv_heads) * s->head_size > 1 << 30) return "the store's heads: at most 2^30 channels a token";
     const uintptr_t el = s->dtype == AVA_BF16 ? 2 : 4;
     if (!aligned(s->k, el) || !aligned(s->v, el)) return "the store's pools must be aligned to their elements";
     return nullptr;
@@ -98,6 +121,7 @@ int ava_paged_plan(int device, void* stream, const int32_t* cached, const int32_
     for (const void* w : words)
         if (!aligned(w, 4)) return fail(AVA_ERR_ARG, call, "the lists must be 4-byte aligned");
     if (!aligned(slot, 8)) return fail(AVA_ERR_ARG, call, "slot must be 8-byte aligned");
+    if (rows > MOST_ROWS || max_tokens > MOST_TOKENS || n_pages > MOST_PAGES) return fail(AVA_NOT_APPLICABLE, call, "at most 2^24 requests, 2^30 tokens and 2^30 pages");
     OnDevice dev(device);
     if (!dev.ok) return fail(AVA_ERR_CUDA, call, NO_DEVICE);
     PlanArgs a{};
@@ -116,6 +140,8 @@ int ava_paged_append(int device, void* stream, const ava_paged_store* store, con
     if (tokens > 0 && (!k || !v || !slot)) return fail(AVA_ERR_ARG, call, "null pointer");
     if (dtype != AVA_F32 && dtype != AVA_BF16) return fail(AVA_ERR_ARG, call, "dtype is AVA_F32 or AVA_BF16");
     if (token_stride < 0 || head_stride < 0) return fail(AVA_ERR_ARG, call, "strides must not be negative");
+    int64_t extents[] = {store->n_pages, store->kv_heads, store->page_size}, strides[] = {store->page_stride, store->head_stride, store->place_stride};
+    if (!distinct(store->head_size, extents, strides)) return fail(AVA_ERR_ARG, call, "a store that is written must not overlap itself");
     const uintptr_t el = dtype == AVA_BF16 ? 2 : 4;
     if (!aligned(k, el) || !aligned(v, el)) return fail(AVA_ERR_ARG, call, "k and v must be aligned to their elements");
     if (!aligned(slot, 8) || !aligned(status, 4)) return fail(AVA_ERR_ARG, call, "slot must be 8-byte and status 4-byte aligned");
@@ -158,11 +184,14 @@ int ava_paged_attend(int device, void* stream, const ava_paged_store* store, con
     for (const void* w : words)
         if (!aligned(w, 4)) return fail(AVA_ERR_ARG, call, "lists, lse and status must be 4-byte aligned");
     if (store->head_size != 32 && store->head_size != 64 && store->head_size != 128) return fail(AVA_NOT_APPLICABLE, call, "head sizes 32, 64 and 128");
+    int64_t extents[] = {max_tokens, heads}, strides[] = {out_token_stride, out_head_stride};
+    if (!distinct(store->head_size, extents, strides)) return fail(AVA_ERR_ARG, call, "out must not overlap itself");
     // the store is read in pieces of 16 bytes
     const int64_t piece = store->dtype == AVA_BF16 ? 8 : 4;
     if (!aligned(store->k, 16) || !aligned(store->v, 16) || store->page_stride % piece || store->head_stride % piece || store->place_stride % piece)
         return fail(AVA_ERR_ARG, call, "the store's pools and strides must be multiples of 16 bytes");
     if (dtype == AVA_BF16 && store->dtype == AVA_F32) return fail(AVA_NOT_APPLICABLE, call, "bf16 queries over an f32 store");
+    if (rows > MOST_ROWS || static_cast<int64_t>(max_tokens) * heads > MOST_TOKENS) return fail(AVA_NOT_APPLICABLE, call, "at most 2^24 requests and 2^30 tokens times heads");
     OnDevice dev(device);
     if (!dev.ok) return fail(AVA_ERR_CUDA, call, NO_DEVICE);
     const int sms = sm_count(device);
@@ -190,7 +219,7 @@ int ava_verify_drafts(int device, void* stream, const float* p, int64_t p_stride
     for (const void* w : words)
         if (!aligned(w, 4)) return fail(AVA_ERR_ARG, call, "arrays must be 4-byte aligned");
     if (!aligned(uniform, 8)) return fail(AVA_ERR_ARG, call, "uniform must be 8-byte aligned");
-    if (vocab > (1 << 30) || rows > (1 << 24)) return fail(AVA_NOT_APPLICABLE, call, "at most 2^30 tokens and 2^24 requests");
+    if (vocab > (1 << 30) || rows > MOST_ROWS) return fail(AVA_NOT_APPLICABLE, call, "a vocabulary of at most 2^30 tokens and 2^24 requests");
     OnDevice dev(device);
     if (!dev.ok) return fail(AVA_ERR_CUDA, call, NO_DEVICE);
     VerifyArgs a{};

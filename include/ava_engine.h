@@ -542,7 +542,7 @@ int ava_paged_plan(int device, void* stream, const int32_t* cached, const int32_
                    uint32_t* status);
 
 /* The keys and values of `tokens` new tokens into the store: k and v (dtype; element (token, head, channel) of either at
- * token * token_stride + head * head_stride + channel) to the places slot[token] names; a negative slot is passed over.  f32 rows may go into
+ * token * token_stride + head * head_stride + channel) to the places slot[token] names (stores and results that overlap themselves are refused); a negative slot is passed over.  f32 rows may go into
  * an f32 or a bf16 store (rounded once, to nearest even), bf16 rows into a bf16 store; else AVA_NOT_APPLICABLE.  Slots are
  * to be distinct: of two tokens with the same slot either's bytes may stay. */
 int ava_paged_append(int device, void* stream, const ava_paged_store* store, const void* k, const void* v, int32_t dtype, int64_t token_stride,
@@ -558,6 +558,7 @@ int ava_paged_append(int device, void* stream, const ava_paged_store* store, con
  * f32; the products run on bf16 tensor cores with f32 operands carried as three bf16 limbs (2^-24 of each), and with
  * bf16 q the softmax weights are rounded to bf16 for their product with the values.  The pools and their strides must be
  * multiples of 16 bytes.  What a request on a page outside the store reads (BAD_PAGE) means nothing.
+ * At most 2^24 requests, 2^30 tokens times heads, and fewer than 2^29 tokens of a request (more: BAD_LENGTH).
  * max_fresh: the largest number of new tokens of a request, as the host knows it; it only chooses the kernel, and a
  * longer request is read in full all the same.  max_tokens: rows of q and out.
  * workspace: ava_paged_attend_workspace(device, head_size) bytes, 16-byte aligned, contents arbitrary and not kept from

@@ -122,6 +122,36 @@ def test_types_and_sizes_that_are_not_covered(L, mem):
     assert L.ava_paged_attend_workspace(0, 48) == -1
 
 
+def test_sizes_beyond_the_kernels_indexes_are_refused(L, mem):
+    for kw in (dict(rows=(1 << 24) + 1), dict(max_tokens=(1 << 30) + 1), dict(n_pages=(1 << 30) + 1)):
+        assert plan(L, mem, **kw) == NOT
+    assert plan(L, mem, rows=1 << 24, max_tokens=1 << 30, n_pages=1 << 30) == CUDA
+    assert attend(L, mem, rows=(1 << 24) + 1) == NOT and attend(L, mem, max_tokens=(1 << 28) + 1) == NOT and attend(L, mem, max_tokens=1 << 28) == CUDA
+    assert verify(L, mem, rows=(1 << 24) + 1) == NOT and verify(L, mem, vocab=(1 << 30) + 1, p_stride=1 << 40, q_stride=1 << 40) == NOT
+    wide = store(mem, kv_heads=1 << 20, head_size=1 << 11, place_stride=1 << 11, head_stride=1 << 14, page_stride=1 << 40)
+    assert append(L, mem, store=wide) == ARG
+
+
+@pytest.mark.parametrize("kw", [dict(page_stride=0), dict(head_stride=0), dict(head_stride=256), dict(page_stride=1023), dict(place_stride=128), dict(place_stride=64, head_stride=64),
+                                dict(page_stride=448, head_stride=512, place_stride=64)])
+def test_a_store_that_overlaps_itself_is_refused_where_it_is_written(L, mem, kw):
+    assert append(L, mem, store=store(mem, **kw)) == ARG
+    assert b"overlap" in L.ava_serving_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(head_stride=64, place_stride=128), dict(page_stride=64, place_stride=256, head_stride=2048), dict(n_pages=1, page_stride=0),
+                                dict(kv_heads=1, head_stride=0)])
+def test_a_store_in_any_order_of_its_dimensions_is_written(L, mem, kw):
+    assert append(L, mem, store=store(mem, **kw)) == CUDA
+
+
+def test_a_result_that_overlaps_itself_is_refused(L, mem):
+    assert attend(L, mem, out_token_stride=0) == ARG and attend(L, mem, out_token_stride=128) == ARG
+    assert attend(L, mem, out_token_stride=64, out_head_stride=16 * 64) == CUDA                 # [heads][tokens][channels]
+    assert attend(L, mem, out_token_stride=0, max_tokens=1) == CUDA and attend(L, mem, out_token_stride=64, heads=2, out_head_stride=64) == ARG
+    assert attend(L, mem, q_token_stride=0, q_head_stride=0) == CUDA                            # read: broadcasts are fine
+
+
 def test_host_tensors_are_refused():
     import torch
     z = torch.zeros(4, dtype=torch.int32)
