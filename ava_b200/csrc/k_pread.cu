@@ -49,6 +49,15 @@ __device__ __forceinline__ void limbs(float a, float b, uint32_t (&l)[3]) {
     l[1] = pack_bf16(a, b);
     l[2] = pack_bf16(__fsub_rn(a, low_half(l[1])), __fsub_rn(b, high_half(l[1])));
 }
+// The same with the first limb rounded towards 0: of a value near the type's largest it stays finite, and so does 0 times it
+// (to nearest it would be infinite, in a place that nobody sees as well).  The other two still leave nothing over.
+__device__ __forceinline__ void limbs_down(float a, float b, uint32_t (&l)[3]) {
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(l[0]) : "f"(b), "f"(a));
+    a = __fsub_rn(a, low_half(l[0]));
+    b = __fsub_rn(b, high_half(l[0]));
+    l[1] = pack_bf16(a, b);
+    l[2] = pack_bf16(__fsub_rn(a, low_half(l[1])), __fsub_rn(b, high_half(l[1])));
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -427,7 +436,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) read_kernel(const __grid_consta
                         const int ch = 16 * mb + 8 * (i & 1) + g, key = 8 * (i >> 1) + 2 * tq;
                         const unsigned char* v = st + St::POOL + (ch & 3) * 4;
                         uint32_t l[LS];
-                        limbs(*reinterpret_cast<const float*>(v + St::at(key, ch / 4)), *reinterpret_cast<const float*>(v + St::at(key + 1, ch / 4)), l);
+                        limbs_down(*reinterpret_cast<const float*>(v + St::at(key, ch / 4)), *reinterpret_cast<const float*>(v + St::at(key + 1, ch / 4)), l);
 #pragma unroll
                         for (int y = 0; y < LS; ++y) vf[y][i] = l[y];
                     }

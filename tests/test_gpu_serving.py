@@ -504,6 +504,25 @@ def test_attend_values_that_are_not_finite_reach_the_rows_that_see_them_only(T, 
         at += f
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("fresh,page,hs", [(1, 16, 32), (5, 24, 64), (9, 8, 128), (200, 16, 64)])
+def test_attend_the_types_largest_values_in_hidden_places_do_not_leak(T, S, dt, fresh, page, hs):
+    """Padding in front of the sequence, and the last new token, which the rows before it do not see."""
+    rng = np.random.default_rng(fresh)
+    x = attend_inputs(T, rng, [(64, fresh), (40, fresh)], 4, 2, hs, page, dt, first=[16, 21])
+    clean = call_attend(T, S, x, 0.125)
+    check_attend(T, x, *clean, 0.125)
+    big = T.finfo(x["kp"].dtype).max
+    for r, hidden in ((0, 16), (1, 21)):
+        last = [64, 40][r] + fresh - 1
+        for j in list(range(hidden)) + [last] * (fresh > 1):
+            at = int(x["table"][r, j // page])
+            x["kp"][at, :, j % page] = x["vp"][at, :, j % page] = -big if j % 2 else big
+    out, lse = call_attend(T, S, x, 0.125)
+    keep = [i for i in range(2 * fresh) if fresh == 1 or i % fresh != fresh - 1]
+    assert T.equal(out[keep], clean[0][keep]) and T.equal(lse[keep], clean[1][keep])
+
+
 def test_attend_takes_offsets_beyond_32_bits(T, S):
     """Pages that lie more than 2^31 elements into the pools (k and v share one)."""
     rng = np.random.default_rng(6)
