@@ -198,7 +198,7 @@ __device__ __forceinline__ uint64_t desc_keys_down(uint32_t at, uint32_t group) 
 }
 
 struct Bars {
-    uint64_t full[10], empty[10], passed[10], q_ready[2], s_ready[2][2], p_ready[2][2], pv_done[2][2], o_free[2];
+    uint64_t full[10], empty[10], passed[10], q_ready[2], s_ready[2][2], p_ready[2][2], pv_done[2][2], o_free[2], drained[2];
     uint32_t tmem, failed;
 };
 static_assert(sizeof(Bars) <= 768, "barriers");
@@ -347,6 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 bar_init(&bars->pv_done[w][i], 1);
             }
             bar_init(&bars->o_free[w], 4);
+            bar_init(&bars->drained[w], 1);
         }
         bars->failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -656,6 +657,9 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     bar_arrive(&bars->empty[slot]);
                 }
             };
+            // (a run without work for this group is passed over only when its rows are done with the one before: the sweeping
+            // warp is then never further ahead of them than the ring)
+            if (from >= to && n_run > 0) ok = ok && warp_wait(&bars->o_free[w], (n_run - 1) & 1, failed);
             for (int t = run.ta; t < min(from, run.tb) && ok; ++t) pass(t);
             if (from < to) ok = ok && warp_wait(&bars->q_ready[w], n_run & 1, failed);
             // a step: the mix of unit t, and as soon as that is done the scores of the unit that takes its place
@@ -709,6 +713,11 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             base += (uint32_t)(run.tb - run.ta);
             u = run.stop;
             if (u < end) next_item(a, it);
+        }
+        if (!ok) {   // the multiplies in flight end before the block does
+            if (elected()) commit(&bars->drained[w]);
+            __syncwarp();
+            bar_wait(&bars->drained[w], 0);
         }
     } else if (warp == 10) {
         // ---- the copies: a lane per box
