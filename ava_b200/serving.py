@@ -48,6 +48,13 @@ def _list(t, name, device, shape=None, dtype=_I32):
     return t.data_ptr()
 
 
+def _word(*values):
+    """Numbers that go into 32 bits (ctypes would cut them)."""
+    for x in values:
+        if not -0x80000000 <= x <= 0x7fffffff:
+            raise ValueError(f"{x} does not fit 32 bits")
+
+
 def _opt(t, name, device, shape=None, dtype=_I32):
     return None if t is None else _list(t, name, device, shape, dtype)
 
@@ -78,6 +85,7 @@ def plan(cached, fresh, table, owned, free_list, free_count, page_size, q_start,
     """The step's lists on the GPU: `table` [rows, max_pages], `owned` [rows] and the stack `free_list` [n_pages] of height
     `free_count` [1] move on (owned and free_count in place unless owned_out / free_count_out are given), `q_start`
     [rows + 1] gets the packed order and `slot` (int64), `pos`, `row` [max_tokens] the tokens' places (-1 behind the last)."""
+    _word(page_size)
     device = _cuda(cached)
     rows, tokens = (cached.shape[0],), slot.shape
     if table.dim() != 2 or table.shape[0] != rows[0]:
@@ -112,7 +120,8 @@ def append(k, v, slot, k_pages, v_pages, *, status=None, stream=None):
 
 def attend_workspace(device, head_size: int) -> int:
     """Bytes of workspace `attend` needs on a device for a head size."""
-    n = engine.lib().ava_paged_attend_workspace(torch.device(device).index or 0, head_size)
+    index = torch.device(device).index
+    n = engine.lib().ava_paged_attend_workspace(torch.cuda.current_device() if index is None else index, head_size)
     if n < 0:
         _fail(engine.ERR_CUDA if head_size in (32, 64, 128) else engine.NOT_APPLICABLE)
     return n
@@ -123,6 +132,7 @@ def attend(q, k_pages, v_pages, table, cached, q_start, out, *, max_fresh, works
     the keys first[r] .. cached[r] + i, of them the last `window` if that is not 0.  out like q; lse [tokens, heads] f32.
     max_fresh: the host's largest number of new tokens per request (chooses the kernel).  workspace: a uint8 tensor of
     attend_workspace() bytes, one for each call that may run at the same time."""
+    _word(max_fresh, window)
     device = _cuda(q)
     store = _store(k_pages, v_pages)
     shape, stride, to = q.shape, q.stride(), out.stride()

@@ -152,6 +152,16 @@ def test_a_result_that_overlaps_itself_is_refused(L, mem):
     assert attend(L, mem, q_token_stride=0, q_head_stride=0) == CUDA                            # read: broadcasts are fine
 
 
+def test_numbers_beyond_32_bits_are_refused():
+    import torch
+    z = torch.zeros(4, dtype=torch.int32)
+    for kw in (dict(window=1 << 32), dict(max_fresh=1 << 31)):
+        with pytest.raises(ValueError, match="32 bits"):
+            serving.attend(z, z, z, z, z, z, z, **{**dict(max_fresh=1, workspace=z, scale=1.0), **kw})
+    with pytest.raises(ValueError, match="32 bits"):
+        serving.plan(z, z, z, z, z, z, (1 << 32) + 16, z, z)
+
+
 def test_host_tensors_are_refused():
     import torch
     z = torch.zeros(4, dtype=torch.int32)
