@@ -55,16 +55,18 @@ struct Found {
     uint64_t keys[15];
 };
 constexpr uint32_t RUNS = 16;
+constexpr uint32_t ROWS_ROOM = 2048;     // bytes
 
 template <int HS_, int L_>
 struct Shape {
     static constexpr int HS = HS_, L = L_;
     static constexpr int HALVES = HS / 64;                           // 64-channel columns of 128 bytes a row
     static constexpr uint32_t Q_LIMB = 128 * HS * 2, Q_TILE = L * Q_LIMB, KV = KT * HS * 2;
-    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 7) : 4;   // units in shared memory
+    static constexpr uint32_t RING = HS == 64 ? (L == 1 ? 10 : 6) : 4;   // units in shared memory
     static constexpr uint32_t OFF_K = 2 * Q_TILE, OFF_V = OFF_K + RING * KV, OFF_BAR = OFF_V + RING * KV;
     static constexpr uint32_t OFF_FOUND = OFF_BAR + 768;             // Found[RUNS]
-    static constexpr uint32_t BYTES = OFF_FOUND + RUNS * sizeof(Found) + 1024;   // the rest: alignment to 1024
+    static constexpr uint32_t OFF_ROWS = (OFF_FOUND + RUNS * (uint32_t)sizeof(Found) + 127) / 128 * 128;   // put_rows' room, ROWS_ROOM for each row warp
+    static constexpr uint32_t BYTES = OFF_ROWS + 8 * ROWS_ROOM + 1024;   // the rest: alignment to 1024
     // Tensor memory of a group: places of scores and weights, the mix.  A place's scores are read a chunk at a time and the
     // weights go back over it: the first limb in its first half, the second in the second, the third outside.
     static __device__ __forceinline__ uint32_t weights_at(int l, int c) { return l == 2 ? 64 + c / 2 : c + CW / 2 * l; }   // of the chunk of keys from c on
@@ -206,6 +208,7 @@ static_assert(sizeof(Bars) <= 768, "barriers");
 // A wait that ends: true when the phase is there, false when it ran out here or anywhere in the block.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
     const uint32_t addr = s32(bar);
+#pragma unroll 1
     for (uint32_t i = 0; i < B_WAIT_LIMIT; ++i) {
         uint32_t done;
         asm volatile(
@@ -245,18 +248,18 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     if ((threadIdx.x & 31) == 0) bar_arrive(bar);
 }
 
-// A worker's run over one stretch: units [ta, tb) of the store's own KT-key units, and of them group w's [a, b).
+// A worker's run over one stretch: units [ta, tb) of the store's own KT-key units, and of them [a, b) for the rows of group w.
 struct Run {
     long long stop;
     bool whole;
     int ta, tb, rows;
-    int a[2], b[2];
-    __device__ __forceinline__ int count(int w) const { return max(b[w] - a[w], 0); }
+    int a, b;
+    __device__ __forceinline__ int count() const { return max(b - a, 0); }
     int all_from, all_to;                // keys that every row of the tile sees
     // whether the sweeping warp goes over unit t: some row does not see all of it
     __device__ __forceinline__ bool swept(int t) const { return t * KT < all_from || t * KT + KT > all_to; }
 };
-__device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, long long u, long long end) {
+__device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, long long u, long long end, int w) {
     Run r;
     const split::Share s = split::share<Plan>(it, u, end);
     r.stop = s.stop;
@@ -267,16 +270,13 @@ __device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, 
     r.rows = min(it.q.f * a.group - it.tile * MR, MR);
     r.all_to = it.q.c + it.tile * MR / a.group + 1;
     r.all_from = a.window > 0 ? max(it.q.first, it.q.c + (it.tile * MR + r.rows - 1) / a.group + 1 - a.window) : it.q.first;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        r.a[w] = r.b[w] = r.ta;
-        if (r.rows > 128 * w) {   // the keys that this group's rows see
-            const int m0 = it.tile * MR + 128 * w, m1 = it.tile * MR + min(r.rows, 128 * w + 128) - 1;
-            const int hi = it.q.c + m1 / a.group + 1, lo = a.window > 0 ? max(it.q.first, it.q.c + m0 / a.group + 1 - a.window) : it.q.first;
-            if (lo < hi) {
-                r.a[w] = max(r.ta, lo / KT);
-                r.b[w] = min(r.tb, (hi + KT - 1) / KT);
-            }
+    r.a = r.b = r.ta;
+    if (r.rows > 128 * w) {   // the keys that this group's rows see
+        const int m0 = it.tile * MR + 128 * w, m1 = it.tile * MR + min(r.rows, 128 * w + 128) - 1;
+        const int hi = it.q.c + m1 / a.group + 1, lo = a.window > 0 ? max(it.q.first, it.q.c + m0 / a.group + 1 - a.window) : it.q.first;
+        if (lo < hi) {
+            r.a = max(r.ta, lo / KT);
+            r.b = min(r.tb, (hi + KT - 1) / KT);
         }
     }
     return r;
@@ -284,11 +284,47 @@ __device__ __forceinline__ Run run_of(const ReadArgs& a, const split::Item& it, 
 
 __device__ __forceinline__ void next_item(const ReadArgs& a, split::Item& it) { split::next<Plan>(a, it); }
 
-// Adds what the sweeping warp has taken out of V to a row that sees it, in its results or in its end (the thread's own
+// PIECES 16-byte pieces of a row per lane, as stores whose lanes lie next to one another: through the warp's shared memory.
+// (A lane storing its own row touches 32 lines with every 16 bytes; the results of a tile took 4100 cycles of the block's
+// load and store unit that way, 1000 this way, and its queries as many.)  at: where the lane's row begins, in bytes; rows: that are stored.
+template <int PIECES>
+__device__ __forceinline__ void put_rows(unsigned char* room, const uint32_t (&x)[4 * PIECES], unsigned char* base, int64_t at, int rows, bool wide, int element) {
+    constexpr int ROW = 16 * PIECES, ROWS = (int)ROWS_ROOM / ROW;
+    const int lane = threadIdx.x & 31;
+    auto turned = [](int row, int piece) { return row * ROW + ((piece ^ (PIECES == 8 ? row & 7 : (row >> 1) & 3)) << 4); };
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += ROWS) {
+        if (lane / ROWS * ROWS == r0) {
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) *reinterpret_cast<uint4*>(room + turned(lane % ROWS, k)) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < ROWS * PIECES / 32; ++i) {
+            const int row = (i * 32 + lane) / PIECES, piece = lane % PIECES;
+            const uint4 y = *reinterpret_cast<const uint4*>(room + turned(row, piece));
+            unsigned char* to = base + __shfl_sync(0xffffffffu, at, r0 + row) + piece * 16;
+            if (r0 + row >= rows) continue;
+            if (wide) {
+                *reinterpret_cast<uint4*>(to) = y;
+            } else {
+                const unsigned char* from = room + turned(row, piece);
+#pragma unroll 1
+                for (int k = 0; k < 16; k += element) {
+                    if (element == 4) *reinterpret_cast<uint32_t*>(to + k) = *reinterpret_cast<const uint32_t*>(from + k);
+                    else *reinterpret_cast<uint16_t*>(to + k) = *reinterpret_cast<const uint16_t*>(from + k);
+                }
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// Adds what the sweeping warp has taken out of V to a row that sees it, in its results or in its end (the warp's own
 // writes): an infinity or a NaN is what its mix then is.
 template <int HS>
-__device__ __noinline__ void add_found(const ReadArgs& a, const split::Item& it, const volatile Found* found, int low, int pos, int from, int to, float* end, int64_t out_at) {
-    const int32_t* pages = a.table + (int64_t)it.r * a.max_pages;
+__device__ __noinline__ void add_found(const ReadArgs& a, int r, int head, const volatile Found* found, int low, int pos, int from, int to, float* end, int64_t out_at) {
+    const int32_t* pages = a.table + (int64_t)r * a.max_pages;
     for (int f = 0; f < found->count; ++f) {
         const int t = found->unit[f];
         if (t < from || t >= to) continue;
@@ -297,7 +333,8 @@ __device__ __noinline__ void add_found(const ReadArgs& a, const split::Item& it,
             if (j < low || j > pos) continue;
             const int page = pages[j / a.s.page_size];
             if (page < 0 || page >= a.s.n_pages) continue;
-            const uint16_t* v = static_cast<const uint16_t*>(a.s.v) + page * a.s.page_stride + it.head * a.s.head_stride + (j % a.s.page_size) * a.s.place_stride;
+            const uint16_t* v = static_cast<const uint16_t*>(a.s.v) + page * a.s.page_stride + head * a.s.head_stride + (j % a.s.page_size) * a.s.place_stride;
+#pragma unroll 1
             for (int c = 0; c < HS; ++c) {
                 if ((v[c] & 0x7f80u) != 0x7f80u) continue;
                 const float x = bf16_to_f(v[c]);
@@ -310,7 +347,7 @@ __device__ __noinline__ void add_found(const ReadArgs& a, const split::Item& it,
 }
 
 template <typename Sh>
-__global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ReadArgs a,
+__global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ReadArgs a,
                                                             const int heads_inside, const int box_rows, float* __restrict__ ends, split::Cut* __restrict__ cuts) {
     constexpr int HS = Sh::HS, L = Sh::L;
     constexpr uint32_t RING = Sh::RING;
@@ -328,10 +365,15 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
     if (bad_length && a.status && blockIdx.x == 0) atomicOr(a.status, AVA_PAGED_BAD_LENGTH);
     const int worker = blockIdx.x;
     const long long per = max((line.total() + gridDim.x - 1) / (long long)gridDim.x, 1ll);
-    split::Item it = {}, after = {};
+    split::Item it = {};
     it.r = -1;
-    long long u = split::piece<Plan>(a, line, per, worker, &it);
-    const long long end = split::piece<Plan>(a, line, per, worker + 1ll, &after, &it);
+    long long u = 0, end = 0;
+#pragma unroll 1
+    for (int k = 1; k >= 0; --k) {           // where the piece ends, then where it begins
+        end = u;
+        const split::Item known = it;
+        u = split::piece<Plan>(a, line, per, worker + k, &it, &known);
+    }
     if (tid == 0) {
         cuts[worker].workers = 0;
         for (uint32_t i = 0; i < RING; ++i) {
@@ -372,70 +414,79 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         const float scale2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;   // its sign is in the queries
         const bool out_wide = !((reinterpret_cast<uintptr_t>(a.out) & 15) || (a.out_token_stride % (L == 3 ? 4 : 8)) || (a.out_head_stride % (L == 3 ? 4 : 8)));
         uint32_t n_p = 0, runs = 0;      // units of this group so far: its barriers' phases; runs with units
-        // A run's queries, a row per thread, into the operand layout.  They are brought as soon as the scores of the run
-        // before are made, in front of its epilogue, so that the first scores of the next run are ready behind it.
-        constexpr int CH = L == 3 ? 4 : 8;   // channels in 16 bytes
+        // A run's queries into the operand layout, the warp's 32 rows together, lanes next to one another reading a row.  They are
+        // brought as soon as the scores of the run before are made, in front of its epilogue, so that the first scores of the
+        // next run are ready behind it.  All of it in small loops: code that runs once a tile comes from beyond the instruction
+        // caches, some five cycles an instruction, and a straight-line form took 7000 cycles a tile.
+        constexpr int EL = L == 3 ? 4 : 2, CH = 16 / EL, PIECES = HS / CH;   // channels in 16 bytes, pieces of a row
         const bool q_wide = !((reinterpret_cast<uintptr_t>(a.q) & 15) || (a.q_token_stride % CH) || (a.q_head_stride % CH));
         // the scale's sign goes into the queries, so that the largest score is the largest product; a scale of 0 empties them
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : 0xffffffffu;
         auto bring = [&](const split::Item& of, const Run& run) {
-            if (run.count(w) == 0) return;
             const int m = of.tile * MR + min(q_row, run.rows - 1), i = m / a.group, h = of.head * a.group + (m - i * a.group);
-            const int64_t from = (int64_t)(of.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride;
-            unsigned char* to = smem + w * Sh::Q_TILE;
+            const int64_t mine_from = ((int64_t)(of.q.start + i) * a.q_token_stride + (int64_t)h * a.q_head_stride) * EL;
+            const int piece = lane % PIECES, r0 = (warp & 3) * 32;
+            // 16 bytes of a row where they will be multiplied from; f32 ones in the first two limbs' places
+            unsigned char* to = smem + w * Sh::Q_TILE + (piece / 8) * (L == 3 ? (int)Sh::Q_LIMB : 128 * 128);
+            const unsigned char* q = static_cast<const unsigned char*>(a.q) + piece * 16;
 #pragma unroll 1
-            for (int c0 = 0; c0 < HS; c0 += 64) {
-                uint4 x[64 / CH];
-#pragma unroll
-                for (int k = 0; k < 64 / CH; ++k) {
-                    const int64_t at = from + c0 + k * CH;
-                    if (q_wide) {
-                        x[k] = *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) + at * (L == 3 ? 4 : 2));
-                    } else if (L == 3) {
-                        const uint32_t* q = static_cast<const uint32_t*>(a.q) + at;
-                        x[k] = make_uint4(q[0], q[1], q[2], q[3]);
-                    } else {
-                        const uint16_t* q = static_cast<const uint16_t*>(a.q) + at;
-                        x[k] = make_uint4(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16), q[4] | ((uint32_t)q[5] << 16), q[6] | ((uint32_t)q[7] << 16));
+            for (int k = 0; k < PIECES; ++k) {
+                const int row = (k * 32 + lane) / PIECES;
+                const unsigned char* from = q + __shfl_sync(0xffffffffu, mine_from, row);
+                unsigned char* at = to + swz128(r0 + row, 8 * (piece % 8));
+                if (q_wide) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s32(at)), "l"(from) : "memory");
+                } else {
+#pragma unroll 1
+                    for (int b = 0; b < 16; b += EL) {
+                        if (EL == 4) *reinterpret_cast<uint32_t*>(at + b) = *reinterpret_cast<const uint32_t*>(from + b);
+                        else *reinterpret_cast<uint16_t*>(at + b) = *reinterpret_cast<const uint16_t*>(from + b);
                     }
                 }
-                unsigned char* at = to + (c0 / 64) * (128 * 128);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if constexpr (L == 3) {
+                unsigned char* limbs_at = smem + w * Sh::Q_TILE;
+#pragma unroll 1
+                for (int k = 0; k < PIECES; ++k) {   // two rows at a time: all of them read, then their limbs written over them
+                    const int row = r0 + (k * 32 + lane) / PIECES;
+                    const uint4 x = *reinterpret_cast<const uint4*>(to + swz128(row, 8 * (piece % 8)));
+                    __syncwarp();
+                    uint64_t y[2] = {two(__uint_as_float(x.x), __uint_as_float(x.y)), two(__uint_as_float(x.z), __uint_as_float(x.w))};
+                    unsigned char* at = limbs_at + swz128(row, 8 * (piece / 2)) + (piece & 1) * 8;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {   // 8 channels: 16 bytes of a limb
-                    if constexpr (L == 3) {
-                        const uint4 u = x[2 * c], v = x[2 * c + 1];
-                        uint64_t y[4] = {two(__uint_as_float(u.x), __uint_as_float(u.y)), two(__uint_as_float(u.z), __uint_as_float(u.w)),
-                                         two(__uint_as_float(v.x), __uint_as_float(v.y)), two(__uint_as_float(v.z), __uint_as_float(v.w))};
-#pragma unroll
-                        for (int l = 0; l < L; ++l) {
-                            uint32_t p[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) p[k] = (limb(y[k]) ^ sign) & keep;
-                            *reinterpret_cast<uint4*>(at + l * Sh::Q_LIMB + swz128(row, 8 * c)) = make_uint4(p[0], p[1], p[2], p[3]);
-                        }
-                    } else {
-                        const uint4 u = x[c];
-                        *reinterpret_cast<uint4*>(at + swz128(row, 8 * c)) = make_uint4((u.x ^ sign) & keep, (u.y ^ sign) & keep, (u.z ^ sign) & keep, (u.w ^ sign) & keep);
+                    for (int l = 0; l < L; ++l) {
+                        const uint32_t p0 = (limb(y[0]) ^ sign) & keep, p1 = (limb(y[1]) ^ sign) & keep;
+                        *reinterpret_cast<uint2*>(at + l * Sh::Q_LIMB) = make_uint2(p0, p1);
                     }
+                }
+            } else if (sign || !keep) {
+#pragma unroll 1
+                for (int k = 0; k < PIECES; ++k) {
+                    uint4* at = reinterpret_cast<uint4*>(to + swz128(r0 + (k * 32 + lane) / PIECES, 8 * (piece % 8)));
+                    const uint4 x = *at;
+                    *at = make_uint4((x.x ^ sign) & keep, (x.y ^ sign) & keep, (x.z ^ sign) & keep, (x.w ^ sign) & keep);
                 }
             }
             fence_async();
             warp_arrive(&bars->q_ready[w]);
         };
-        if (u < end) bring(it, run_of(a, it, u, end));
-        while (u < end && ok) {
-            const Run run = run_of(a, it, u, end);
+        // (the first time round there is no run yet, only the next one's queries: one place for them in the code)
+        bool none_yet = true;
+        Run run = {};
+        run.stop = u;
+        while (ok && (none_yet || u < end)) {
             const bool whole = run.whole;
-            const int units = run.count(w);
+            const int units = run.count();
             const bool live = q_row < run.rows;
-            const int m = it.tile * MR + min(q_row, run.rows - 1), i = m / a.group, h = it.head * a.group + (m - i * a.group);
+            const int m = it.tile * MR + max(min(q_row, run.rows - 1), 0), i = m / a.group, h = it.head * a.group + (m - i * a.group);
             const int pos = it.q.c + i, low = a.window > 0 ? max(it.q.first, pos - a.window + 1) : it.q.first;
             float top = -INFINITY, sum = 0.0f;
             uint64_t acc[FLUSH ? HS / 2 : 1];    // the mix of the units that have been flushed
 #pragma unroll
             for (int k = 0; k < (FLUSH ? HS / 2 : 1); ++k) acc[k] = 0ull;
             for (int n = 0; n < units && ok; ++n) {
-                const int t = run.a[w] + n;
+                const int t = run.a + n;
                 const uint32_t place = n_p % PLACES, at = mine + place * Sh::PLACE;
                 ok = warp_wait(&bars->s_ready[w][place], (n_p / PLACES) & 1, failed);
                 if (!ok) break;
@@ -539,17 +590,20 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 ++n_p;
             }
             if (!ok) break;
+            split::Item then = it;
+            Run then_run = run;
             if (run.stop < end) {
-                split::Item then = it;
-                next_item(a, then);
-                bring(then, run_of(a, then, run.stop, end));
+                if (!none_yet) next_item(a, then);
+                then_run = run_of(a, then, run.stop, end, w);
+                if (then_run.count() > 0) bring(then, then_run);
             }
             // ---- the read of the row, or this piece's end of it
             if (units > 0 && ok) ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
             if (!ok) break;
             tc_after();
-            {
+            if (!none_yet) {
                 const float inv = whole ? (sum > 0.0f ? 1.0f / sum : sum) : 1.0f;
+                unsigned char* room = smem + Sh::OFF_ROWS + warp * ROWS_ROOM;
                 float* end_of = ends + ((int64_t)worker * 2 + (u == it.begin ? 1 : 0)) * Ends<HS, MR>::FLOATS;
                 const int64_t to = (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride;
 #pragma unroll(FLUSH ? HS / 32 : 1)
@@ -571,40 +625,17 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     }
 #pragma unroll
                     for (int k = 0; k < 32; ++k) x[k] = units > 0 ? __uint_as_float(o[k]) : 0.0f;
-                    if (!live) continue;
-                    if (!whole) {
+                    const int rows = run.rows - (q_row - lane);   // of this warp that are there
+                    if (L == 3 || !whole) {
+                        uint32_t y[32];
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(end_of + q_row * HS + c + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
-                    } else if constexpr (L == 3) {
-                        float* out = static_cast<float*>(a.out) + to + c;
-#pragma unroll
-                        for (int k = 0; k < 32; k += 4) {
-                            if (out_wide) *reinterpret_cast<float4*>(out + k) = make_float4(x[k] * inv, x[k + 1] * inv, x[k + 2] * inv, x[k + 3] * inv);
-                            else {
-                                out[k] = x[k] * inv;
-                                out[k + 1] = x[k + 1] * inv;
-                                out[k + 2] = x[k + 2] * inv;
-                                out[k + 3] = x[k + 3] * inv;
-                            }
-                        }
+                        for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(x[k] * inv);
+                        put_rows<8>(room, y, reinterpret_cast<unsigned char*>(whole ? a.out : end_of), 4 * (whole ? to + c : (int64_t)(q_row * HS + c)), rows, !whole || out_wide, 4);
                     } else {
-                        uint16_t* out = static_cast<uint16_t*>(a.out) + to + c;
+                        uint32_t y[16];
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            uint4 v;
-                            v.x = pack_bf16(x[k] * inv, x[k + 1] * inv);
-                            v.y = pack_bf16(x[k + 2] * inv, x[k + 3] * inv);
-                            v.z = pack_bf16(x[k + 4] * inv, x[k + 5] * inv);
-                            v.w = pack_bf16(x[k + 6] * inv, x[k + 7] * inv);
-                            if (out_wide) *reinterpret_cast<uint4*>(out + k) = v;
-                            else {
-                                const uint32_t y[4] = {v.x, v.y, v.z, v.w};
-                                for (int z = 0; z < 4; ++z) {
-                                    out[k + 2 * z] = (uint16_t)y[z];
-                                    out[k + 2 * z + 1] = (uint16_t)(y[z] >> 16);
-                                }
-                            }
-                        }
+                        for (int k = 0; k < 16; ++k) y[k] = pack_bf16(x[2 * k] * inv, x[2 * k + 1] * inv);
+                        put_rows<4>(room, y, static_cast<unsigned char*>(a.out), 2 * (to + c), rows, out_wide, 2);
                     }
                 }
                 if (live) {
@@ -623,11 +654,12 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     cuts[worker].workers = (int)split::last_worker<Plan>(it, per) - worker + 1;
                 }
             }
-            if (units > 0 && live && (run.swept(run.a[w]) || run.swept(run.b[w] - 1))) {
+            __syncwarp();                        // the row's results have been stored by all lanes
+            if (units > 0 && live && (run.swept(run.a) || run.swept(run.b - 1))) {
                 const volatile Found* found = reinterpret_cast<const Found*>(smem + Sh::OFF_FOUND) + runs % RUNS;
                 if (found->count > 0) {          // values that are not finite have been taken out: the row gets those that it sees
                     float* row_end = ends + ((int64_t)worker * 2 + (u == it.begin ? 1 : 0)) * Ends<HS, MR>::FLOATS + q_row * HS;
-                    add_found<HS>(a, it, found, low, pos, run.a[w], run.b[w], whole ? nullptr : row_end,
+                    add_found<HS>(a, it.r, it.head, found, low, pos, run.a, run.b, whole ? nullptr : row_end,
                                   (int64_t)(it.q.start + i) * a.out_token_stride + (int64_t)h * a.out_head_stride);
                 }
             }
@@ -635,7 +667,9 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             tc_before();
             if (units > 0) warp_arrive(&bars->o_free[w]);
             u = run.stop;
-            if (u < end) next_item(a, it);
+            it = then;
+            run = then_run;
+            none_yet = false;
         }
     } else if (warp < 10) {
         // ---- a group's multiplies: one lane issues
@@ -644,8 +678,8 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         const uint32_t d = tmem + w * Sh::GROUP;
         uint32_t n_s = 0, n_p = 0, n_run = 0, base = 0;   // units scored, mixed; runs; units of the ring before this run
         while (u < end && ok) {
-            const Run run = run_of(a, it, u, end);
-            const int from = run.a[w], to = run.b[w];
+            const Run run = run_of(a, it, u, end, w);
+            const int from = run.a, to = run.b;
             auto full = [&](int t) {             // unit t has landed
                 const uint32_t seq = base + (uint32_t)(t - run.ta);
                 ok = ok && warp_wait(&bars->full[seq % RING], (seq / RING) & 1, failed);
@@ -725,7 +759,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         bool bad_page = false;
         const int boxes = KT / box_rows * Sh::HALVES;
         while (u < end && ok) {
-            const Run run = run_of(a, it, u, end);
+            const Run run = run_of(a, it, u, end, 0);
             const int32_t* pages = a.table + (int64_t)it.r * a.max_pages;
             for (int t = run.ta; t < run.tb && ok; ++t, ++n) {
                 // a box is box_rows keys of one page (a unit's keys may lie within one page or run over several)
@@ -764,7 +798,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
         // ---- the sweeping warp
         uint32_t n = 0, runs = 0;
         while (u < end && ok) {
-            const Run run = run_of(a, it, u, end);
+            const Run run = run_of(a, it, u, end, 0);
             volatile Found* found = reinterpret_cast<Found*>(smem + Sh::OFF_FOUND) + runs % RUNS;
             int count = 0;
             for (int t = run.ta; t < run.tb && ok; ++t, ++n) {
