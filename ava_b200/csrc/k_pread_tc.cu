@@ -40,8 +40,9 @@ using namespace tcc;
 
 constexpr int THREADS = 384;             // two groups of 128 rows, a warp per group that issues multiplies, the copies' warp, the sweeping one
 constexpr uint32_t PLACES = 2;           // of scores and weights, per group
-struct Plan {                            // of the line: a tile's queries and results take as long as four units
-    static constexpr int MR = 256, KT = 64, START = 4, SNAP = 4;
+struct Plan {                            // of the line: a tile's queries and results take as long as some units (4: 225 and 587 us, 8: 215 and
+                                         // 582 us for 16 x 1024 and 4 x 2048 new tokens)
+    static constexpr int MR = 256, KT = 64, START = 8, SNAP = 4;
 };
 constexpr int MR = Plan::MR, KT = Plan::KT;
 constexpr float GROWN = 8.0f;            // powers of two a maximum may grow by before the sums are rescaled
@@ -205,8 +206,9 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 768, "barriers");
 
-// A wait that ends: true when the phase is there, false when it ran out here or anywhere in the block.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
+// A wait that ends: true when the phase is there, false when it ran out here or anywhere in the block.  The first look is made
+// in place; the waiting itself is one piece of code for all (in every place it was a third of the kernel's code).
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
     const uint32_t addr = s32(bar);
 #pragma unroll 1
     for (uint32_t i = 0; i < B_WAIT_LIMIT; ++i) {
@@ -226,6 +228,17 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile ui
     }
     *failed = 1;
     return false;
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* failed) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(s32(bar)), "r"(parity)
+        : "memory");
+    return done ? true : wait_slow(bar, parity, failed);
 }
 // one lane of a whole warp
 __device__ __forceinline__ bool elected() {
@@ -448,17 +461,25 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
             if constexpr (L == 3) {
                 unsigned char* limbs_at = smem + w * Sh::Q_TILE;
 #pragma unroll 1
-                for (int k = 0; k < PIECES; ++k) {   // two rows at a time: all of them read, then their limbs written over them
-                    const int row = r0 + (k * 32 + lane) / PIECES;
-                    const uint4 x = *reinterpret_cast<const uint4*>(to + swz128(row, 8 * (piece % 8)));
-                    __syncwarp();
-                    uint64_t y[2] = {two(__uint_as_float(x.x), __uint_as_float(x.y)), two(__uint_as_float(x.z), __uint_as_float(x.w))};
-                    unsigned char* at = limbs_at + swz128(row, 8 * (piece / 2)) + (piece & 1) * 8;
+                for (int k = 0; k < PIECES; k += 2) {   // four rows at a time: all of them read, then their limbs written over them
+                    uint4 x[2];
 #pragma unroll
-                    for (int l = 0; l < L; ++l) {
-                        const uint32_t p0 = (limb(y[0]) ^ sign) & keep, p1 = (limb(y[1]) ^ sign) & keep;
-                        *reinterpret_cast<uint2*>(at + l * Sh::Q_LIMB) = make_uint2(p0, p1);
+                    for (int z = 0; z < 2; ++z) x[z] = *reinterpret_cast<const uint4*>(to + swz128(r0 + ((k + z) * 32 + lane) / PIECES, 8 * (piece % 8)));
+                    __syncwarp();
+                    uint64_t y[2][2];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        y[z][0] = two(__uint_as_float(x[z].x), __uint_as_float(x[z].y));
+                        y[z][1] = two(__uint_as_float(x[z].z), __uint_as_float(x[z].w));
                     }
+#pragma unroll
+                    for (int l = 0; l < L; ++l)
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            unsigned char* at = limbs_at + l * Sh::Q_LIMB + swz128(r0 + ((k + z) * 32 + lane) / PIECES, 8 * (piece / 2)) + (piece & 1) * 8;
+                            const uint32_t p0 = (limb(y[z][0]) ^ sign) & keep, p1 = (limb(y[z][1]) ^ sign) & keep;
+                            *reinterpret_cast<uint2*>(at) = make_uint2(p0, p1);
+                        }
                 }
             } else if (sign || !keep) {
 #pragma unroll 1
