@@ -514,32 +514,91 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                 tc_after();
                 const int from = low - t * KT, to = pos - t * KT;   // keys [from, to] of the unit are seen
                 const bool edge = __any_sync(0xffffffffu, from > 0 || to < KT - 1);
-                float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                // Both passes over the row go 32 columns at a time, in loops that are not unrolled: straight through, the code is
-                // larger than the instruction caches keep at hand.
+                const uint64_t scales = two(scale2, scale2);
+                uint64_t part[2];
+                if constexpr (L == 1) {
+                    // One pass with the maximum as it was, the weights kept in registers; only when that has grown by more than
+                    // 2^GROWN (a tile's first unit, hardly ever after) a second one with the new maximum.  (Two passes over the
+                    // scores, the maximum first: 579 us for 4 x 2048 new tokens, one 557.)
+                    uint32_t p[KT / 2];
 #pragma unroll 1
-                for (int c = 0; c < KT; c += CW) {
-                    uint32_t s[CW];
-                    tmem_read(at + c, s);
-                    tmem_wait_ld();
-                    if (edge) {
+                    for (bool again = false;; again = true) {
+                        const float base = top == -INFINITY ? 0.0f : top;
+                        const uint64_t bases = two(-base, -base);
+                        float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        part[0] = part[1] = 0ull;
 #pragma unroll
-                        for (int j = 0; j < CW; ++j)
-                            if (c + j < from || c + j > to) s[j] = 0xff800000u;
+                        for (int c = 0; c < KT; c += 32) {
+                            uint32_t s[32];
+                            tmem_ld32(at + c, s);
+                            tmem_wait_ld();
+                            if (edge) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (c + j < from || c + j > to) s[j] = 0xff800000u;
+                            }
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                high[k & 3] = fmaxf(high[k & 3], fmaxf(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])));
+                                float x, y;
+                                apart(fma2(two(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scales, bases), x, y);
+                                x = exp2_fast(x);
+                                y = exp2_fast(y);
+                                part[k & 1] = add2(part[k & 1], two(x, y));
+                                p[c / 2 + k] = pack_bf16(x, y);
+                            }
+                        }
+                        if (again) break;
+                        const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
+                        const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
+                        if (!__any_sync(0xffffffffu, grown)) break;
+                        const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
+                        if (n > 0) {                 // once the unit before has been added up
+                            ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
+                            if (!ok) break;
+                            tc_after();
+#pragma unroll 1
+                            for (int c = 0; c < HS; c += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(mine + Sh::C_O + c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tmem_st32(mine + Sh::C_O + c, o);
+                            }
+                        }
+                        sum *= f;
+                        top = now;
                     }
-#pragma unroll
-                    for (int j = 0; j < CW; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
-                }
-                const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
-                const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
-                const bool due = FLUSH && n > 0 && n % (FLUSH ? FLUSH : 1) == 0;
-                const bool some = __any_sync(0xffffffffu, grown);
-                if (n > 0 && (due || some)) {    // once the unit before has been added up
-                    ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
                     if (!ok) break;
-                    tc_after();
-                }
-                if constexpr (FLUSH > 0) {
+                    tmem_st16(at + Sh::weights_at(0, 0), p);
+                    tmem_st16(at + Sh::weights_at(0, 32), p + 16);
+                } else {
+                    float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    // Two passes, each CW columns at a time in a loop that is not unrolled: straight through, the code is larger than
+                    // the instruction caches keep at hand, and three limbs of 64 weights are more than the registers hold.
+#pragma unroll 1
+                    for (int c = 0; c < KT; c += CW) {
+                        uint32_t s[CW];
+                        tmem_read(at + c, s);
+                        tmem_wait_ld();
+                        if (edge) {
+#pragma unroll
+                            for (int j = 0; j < CW; ++j)
+                                if (c + j < from || c + j > to) s[j] = 0xff800000u;
+                        }
+#pragma unroll
+                        for (int j = 0; j < CW; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
+                    }
+                    const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
+                    const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
+                    const bool due = n > 0 && n % FLUSH == 0;
+                    const bool some = __any_sync(0xffffffffu, grown);
+                    if (n > 0 && (due || some)) {    // once the unit before has been added up
+                        ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
+                        if (!ok) break;
+                        tc_after();
+                    }
                     if (due) {                   // the mix so far joins acc; the next one starts anew
 #pragma unroll
                         for (int c = 0; c < HS; c += 32) {
@@ -550,57 +609,51 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                             for (int k = 0; k < 16; ++k) acc[c / 2 + k] = add2(acc[c / 2 + k], two(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])));
                         }
                     }
-                }
-                if (some) {
-                    const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
-                    if (n > 0 && !due) {
+                    if (some) {
+                        const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
+                        if (n > 0 && !due) {
 #pragma unroll 1
-                        for (int c = 0; c < HS; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(mine + Sh::C_O + c, o);
-                            tmem_wait_ld();
+                            for (int c = 0; c < HS; c += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(mine + Sh::C_O + c, o);
+                                tmem_wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                            tmem_st32(mine + Sh::C_O + c, o);
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tmem_st32(mine + Sh::C_O + c, o);
+                            }
                         }
-                    }
-                    if constexpr (FLUSH > 0) {
 #pragma unroll
                         for (int k = 0; k < HS / 2; ++k) acc[k] = mul2(acc[k], two(f, f));
+                        sum *= f;
+                        top = now;
                     }
-                    sum *= f;
-                    top = now;
-                }
-                const float base = top == -INFINITY ? 0.0f : top;
-                const uint64_t scales = two(scale2, scale2), bases = two(-base, -base);
-                uint64_t part[2] = {0ull, 0ull};
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    const uint64_t bases = two(-base, -base);
+                    part[0] = part[1] = 0ull;
 #pragma unroll 1
-                for (int c = 0; c < KT; c += CW) {
-                    uint32_t s[CW], p[L][CW / 2];
-                    tmem_read(at + c, s);
-                    tmem_wait_ld();
-                    if (edge) {
+                    for (int c = 0; c < KT; c += CW) {
+                        uint32_t s[CW], p[L][CW / 2];
+                        tmem_read(at + c, s);
+                        tmem_wait_ld();
+                        if (edge) {
 #pragma unroll
-                        for (int j = 0; j < CW; ++j)
-                            if (c + j < from || c + j > to) s[j] = 0xff800000u;
-                    }
+                            for (int j = 0; j < CW; ++j)
+                                if (c + j < from || c + j > to) s[j] = 0xff800000u;
+                        }
 #pragma unroll
-                    for (int k = 0; k < CW / 2; ++k) {
-                        float x, y;
-                        apart(fma2(two(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scales, bases), x, y);
-                        x = exp2_fast(x);
-                        y = exp2_fast(y);
-                        uint64_t e = two(x, y);
-                        part[k & 1] = add2(part[k & 1], e);
-                        if constexpr (L == 1) {
-                            p[0][k] = pack_bf16(x, y);
-                        } else {
+                        for (int k = 0; k < CW / 2; ++k) {
+                            float x, y;
+                            apart(fma2(two(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scales, bases), x, y);
+                            x = exp2_fast(x);
+                            y = exp2_fast(y);
+                            uint64_t e = two(x, y);
+                            part[k & 1] = add2(part[k & 1], e);
 #pragma unroll
                             for (int l = 0; l < L; ++l) p[l][k] = limb(e);
                         }
-                    }
 #pragma unroll
-                    for (int l = 0; l < L; ++l) tmem_write(at + Sh::weights_at(l, c), p[l]);
+                        for (int l = 0; l < L; ++l) tmem_write(at + Sh::weights_at(l, c), p[l]);
+                    }
                 }
                 float x, y;
                 apart(add2(part[0], part[1]), x, y);
