@@ -592,26 +592,15 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     }
                     const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
                     const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
-                    const bool due = n > 0 && n % FLUSH == 0;
                     const bool some = __any_sync(0xffffffffu, grown);
-                    if (n > 0 && (due || some)) {    // once the unit before has been added up
+                    if (n > 0 && some) {             // once the unit before has been added up
                         ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
                         if (!ok) break;
                         tc_after();
                     }
-                    if (due) {                   // the mix so far joins acc; the next one starts anew
-#pragma unroll
-                        for (int c = 0; c < HS; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(mine + Sh::C_O + c, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) acc[c / 2 + k] = add2(acc[c / 2 + k], two(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])));
-                        }
-                    }
                     if (some) {
                         const float now = grown ? peak2 : top, f = grown ? (top == -INFINITY ? 0.0f : exp2_fast(top - now)) : 1.0f;
-                        if (n > 0 && !due) {
+                        if (n > 0) {
 #pragma unroll 1
                             for (int c = 0; c < HS; c += 32) {
                                 uint32_t o[32];
@@ -621,6 +610,7 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                                 for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
                                 tmem_st32(mine + Sh::C_O + c, o);
                             }
+                            tmem_wait_st();          // it may be read again below
                         }
 #pragma unroll
                         for (int k = 0; k < HS / 2; ++k) acc[k] = mul2(acc[k], two(f, f));
@@ -653,6 +643,19 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                         }
 #pragma unroll
                         for (int l = 0; l < L; ++l) tmem_write(at + Sh::weights_at(l, c), p[l]);
+                    }
+                    if (n > 0 && n % FLUSH == 0) {   // the mix so far joins acc; the next one starts anew
+                        ok = warp_wait(&bars->pv_done[w][(n_p - 1) % PLACES], ((n_p - 1) / PLACES) & 1, failed);
+                        if (!ok) break;
+                        tc_after();
+#pragma unroll
+                        for (int c = 0; c < HS; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(mine + Sh::C_O + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) acc[c / 2 + k] = add2(acc[c / 2 + k], two(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])));
+                        }
                     }
                 }
                 float x, y;
