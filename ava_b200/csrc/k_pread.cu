@@ -14,6 +14,11 @@
 // f32 queries, f32 stores and the softmax weights of f32 queries are three bf16 limbs each (2^-24 of the value; a store's
 // are made as its elements come out of shared memory), and of two limbed operands' nine products the six down to 2^-18 are
 // taken.  Two limbs (2^-17) were not enough: an error of 2e-6 of the read where f32 sums leave 5e-7.
+// Measured (one B200, 6.57 TB/s copy): one token of 256 sequences of 1024 to 2048 keys, 12 heads of 64, f32 over bf16: 183 us
+// for 1.12 GB, 0.93 of the copy rate; one token over 131072 keys 75 us, 0.82 (9 us pass until the first keys are multiplied,
+// 5 us join the parts); drafted runs of up to 6 tokens of 64 requests over 8192 keys, 32 heads on 8 of 128, bf16: 257 us for
+// 1.52 GB, 0.90.  Three short requests: 14.5 us, of which 4 lie before the first fetch (lengths, the line, the piece), 4 in
+// the steps of one warp after another, 2 around the join.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

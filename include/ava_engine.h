@@ -557,7 +557,8 @@ int ava_paged_append(int device, void* stream, const ava_paged_store* store, con
  * f32, f32 with bf16, bf16 with bf16; head sizes 32, 64 and 128; else AVA_NOT_APPLICABLE.  Sums, maxima and the mix are
  * f32; the products run on bf16 tensor cores with f32 operands carried as three bf16 limbs (2^-24 of each), and with
  * bf16 q the softmax weights are rounded to bf16 for their product with the values.  The pools and their strides must be
- * multiples of 16 bytes.  What a request on a page outside the store reads (BAD_PAGE) means nothing.
+ * multiples of 16 bytes.  Keys and values that are not finite reach only the tokens that see them; in places that nobody
+ * sees anything may lie.  A table may name a page twice, in one request or in several.  What a request on a page outside the store reads (BAD_PAGE) means nothing.
  * At most 2^24 requests, 2^30 tokens times heads, and fewer than 2^29 tokens of a request (more: BAD_LENGTH).
  * max_fresh: the largest number of new tokens of a request, as the host knows it; it only chooses the kernel, and a
  * longer request is read in full all the same.  max_tokens: rows of q and out.

@@ -523,6 +523,23 @@ def test_attend_the_types_largest_values_in_hidden_places_do_not_leak(T, S, dt, 
     assert T.equal(out[keep], clean[0][keep]) and T.equal(lse[keep], clean[1][keep])
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("fresh", [1, 6, 150])
+def test_attend_pages_that_requests_share(T, S, dt, fresh):
+    """Two requests behind the same stored pages, and a request whose table names one page over and over."""
+    rng = np.random.default_rng(fresh)
+    x = attend_inputs(T, rng, [(64, fresh), (64, fresh), (80, fresh)], 8, 2, 64, 16, dt)
+    table = x["table"]
+    table[1, :4] = table[0, :4]
+    table[2, :5] = table[2, 0].clone()
+    for which in ("ks", "vs"):
+        x[which][1][:, :64] = x[which][0][:, :64]
+        for i in range(1, 5):
+            x[which][2][:, 16 * i:16 * i + 16] = x[which][2][:, :16]
+    out, lse = call_attend(T, S, x, 0.125)
+    check_attend(T, x, out, lse, 0.125)
+
+
 def test_attend_takes_offsets_beyond_32_bits(T, S):
     """Pages that lie more than 2^31 elements into the pools (k and v share one)."""
     rng = np.random.default_rng(6)
