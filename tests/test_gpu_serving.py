@@ -524,6 +524,29 @@ def test_attend_the_types_largest_values_in_hidden_places_do_not_leak(T, S, dt, 
 
 
 @pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("hs,fresh", [(32, 1), (64, 2), (64, 150), (128, 70)])
+@pytest.mark.parametrize("scale", [0.125, -0.3, 0.0])
+def test_attend_queries_and_results_at_odd_addresses(T, S, dt, hs, fresh, scale):
+    """Rows that begin at any element and lie any distance apart: the aligned call's results, and nothing between them touched."""
+    rng = np.random.default_rng(fresh + hs)
+    x = attend_inputs(T, rng, [(70, fresh), (0, fresh), (33, 1)], 4, 2, hs, 16, dt)
+    want = call_attend(T, S, x, scale)
+    check_attend(T, x, *want, scale)
+    q = x["q"]
+    shape, strides = q.shape, (4 * (hs + 5) + 3, hs + 5, 1)
+    odd = lambda t: T.as_strided(t, shape, strides, 1)  # noqa: E731
+    n = shape[0] * strides[0] + 8
+    q_room, out_room = T.zeros(n, dtype=q.dtype, device="cuda:0"), T.full((n,), 7.0, dtype=q.dtype, device="cuda:0")
+    odd(q_room).copy_(q)
+    lse = T.empty_like(want[1])
+    room = T.zeros(S.attend_workspace("cuda:0", hs), dtype=T.uint8, device="cuda:0")
+    S.attend(odd(q_room), x["kp"], x["vp"], x["table"], x["cached"], x["start"], odd(out_room), max_fresh=fresh, workspace=room, scale=scale, lse=lse)
+    assert T.equal(odd(out_room), want[0]) and T.equal(lse, want[1])
+    odd(out_room).fill_(7.0)
+    assert (out_room == 7).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("fresh", [1, 6, 150])
 def test_attend_pages_that_requests_share(T, S, dt, fresh):
     """Two requests behind the same stored pages, and a request whose table names one page over and over."""
