@@ -582,20 +582,20 @@ __global__ void __launch_bounds__(THREADS, 1) read_tc_kernel(const __grid_consta
                     tmem_st16(at + Sh::weights_at(0, 32), p + 16);
                 } else {
                     float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    // Two passes, each CW columns at a time in a loop that is not unrolled: straight through, the code is larger than
+                    // Two passes, some columns at a time in loops that are not unrolled: straight through, the code is larger than
                     // the instruction caches keep at hand, and three limbs of 64 weights are more than the registers hold.
 #pragma unroll 1
-                    for (int c = 0; c < KT; c += CW) {
-                        uint32_t s[CW];
+                    for (int c = 0; c < KT; c += 32) {
+                        uint32_t s[32];
                         tmem_read(at + c, s);
                         tmem_wait_ld();
                         if (edge) {
 #pragma unroll
-                            for (int j = 0; j < CW; ++j)
+                            for (int j = 0; j < 32; ++j)
                                 if (c + j < from || c + j > to) s[j] = 0xff800000u;
                         }
 #pragma unroll
-                        for (int j = 0; j < CW; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
+                        for (int j = 0; j < 32; ++j) high[j & 3] = fmaxf(high[j & 3], __uint_as_float(s[j]));
                     }
                     const float peak2 = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * scale2;
                     const bool grown = peak2 > top + GROWN || (top == -INFINITY && peak2 > -INFINITY);
