@@ -21,12 +21,13 @@
 // accumulators are not ordered by their issue).  Each group has an issuing warp of its own that waits where it must; one
 // warp polling for both took 1500 cycles a round of its own code.
 // Measured (one B200): 4 chunks of up to 2048 tokens over 8192 keys, 32 heads on 8 key heads of 128, bf16: 555 us, 1.05
-// PFLOP/s, 0.64 of the measured bf16 rate; what bounds it is the row threads' instructions (a unit of 64 keys of both
-// groups: 1280 cycles of multiplies, about 1900 in all; a quarter of the exponentials as polynomials in f32 arithmetic
-// made it 15 us slower, so it is not the exponential unit).  16 chunks of up to 1024 over 2048 keys, 12 heads of 64, f32
-// queries: 212 us, three products for each of the 38 GFLOP; bounded by the limbs' instructions as well.  In both the code
+// PFLOP/s, 0.64 of the measured bf16 rate; what bounds it is the latency of the row threads' chain, of which a scheduler has
+// two warps (it issues in 0.41 of the cycles; a unit of 64 keys of both groups: 1280 cycles of multiplies, about 1900 in all; a
+// quarter of the exponentials as polynomials in f32 arithmetic made it 15 us slower, so it is not the exponential unit).
+// 16 chunks of up to 1024 over 2048 keys, 12 heads of 64, f32 queries: 211 us, three products for each of the 38 GFLOP;
+// bounded by the same chain, longer by the limbs.  In both the code
 // a tile runs once costs about five cycles an instruction (it is not in the instruction caches by then), hence the small
-// loops around queries and results and one piece of code for every wait: 213 KB of code and 250 us before, 120 KB and 212 us.
+// loops around queries and results and one piece of code for every wait: 213 KB of code and 250 us before, 120 KB and 211 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
