@@ -43,20 +43,29 @@ def _fail(rc):
 
 def _list(t, name, device, shape=None, dtype=_I32):
     """A contiguous tensor's address."""
-    if t.device != device or not (t.dtype in dtype if isinstance(dtype, tuple) else t.dtype is dtype) or not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise ValueError(f"{name}: contiguous, {dtype}{'' if shape is None else f', shape {tuple(shape)}'}, on {device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.device == device and t.is_contiguous() and (shape is None or t.shape == shape):
+        return t.data_ptr()
+    raise ValueError(f"{name}: contiguous, {dtype}{'' if shape is None else f', shape {tuple(shape)}'}, on {device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _word(*values):
-    """Numbers that go into 32 bits (ctypes would cut them)."""
-    for x in values:
-        if not -0x80000000 <= x <= 0x7fffffff:
-            raise ValueError(f"{x} does not fit 32 bits")
+def _words(t, name, device, shape=None):
+    """The same of 32-bit words, signed or not."""
+    return _list(t, name, device, shape, t.dtype if t.dtype in _WORD else _WORD)
+
+
+_MOST = 0x7fffffff   # of numbers that go into 32 bits: ctypes would cut them
+
+
+def _too_wide(*values):
+    raise ValueError(f"{values}: do not fit 32 bits")
 
 
 def _opt(t, name, device, shape=None, dtype=_I32):
     return None if t is None else _list(t, name, device, shape, dtype)
+
+
+def _status(t, device):
+    return None if t is None else _words(t, "status", device, (1,))
 
 
 def _cuda(t):
@@ -85,7 +94,8 @@ def plan(cached, fresh, table, owned, free_list, free_count, page_size, q_start,
     """The step's lists on the GPU: `table` [rows, max_pages], `owned` [rows] and the stack `free_list` [n_pages] of height
     `free_count` [1] move on (owned and free_count in place unless owned_out / free_count_out are given), `q_start`
     [rows + 1] gets the packed order and `slot` (int64), `pos`, `row` [max_tokens] the tokens' places (-1 behind the last)."""
-    _word(page_size)
+    if not -_MOST <= page_size <= _MOST:
+        _too_wide(page_size)
     device = _cuda(cached)
     rows, tokens = (cached.shape[0],), slot.shape
     if table.dim() != 2 or table.shape[0] != rows[0]:
@@ -95,8 +105,7 @@ def plan(cached, fresh, table, owned, free_list, free_count, page_size, q_start,
         _list(table, "table", device), table.shape[1], _list(owned, "owned", device, rows), _list(owned if owned_out is None else owned_out, "owned_out", device, rows),
         _list(free_list, "free_list", device), _list(free_count, "free_count", device, (1,)),
         _list(free_count if free_count_out is None else free_count_out, "free_count_out", device, (1,)), bool(trim), _list(q_start, "q_start", device, (rows[0] + 1,)),
-        _list(slot, "slot", device, None, _I64), _opt(pos, "pos", device, tokens), _opt(row, "row", device, tokens), tokens[0],
-        _opt(status, "status", device, (1,), _WORD))
+        _list(slot, "slot", device, None, _I64), _opt(pos, "pos", device, tokens), _opt(row, "row", device, tokens), tokens[0], _status(status, device))
     if rc:
         _fail(rc)
 
@@ -113,7 +122,7 @@ def append(k, v, slot, k_pages, v_pages, *, status=None, stream=None):
     if (v.stride() != stride and shape[0]) or (stride[2] != 1 and shape[2] != 1):
         raise ValueError("k and v: the same strides, adjacent channels")
     rc = engine.lib().ava_paged_append(device.index, _stream(stream, device), C.byref(store), k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], stride[0], stride[1],
-                                       _list(slot, "slot", device, None, _I64), shape[0], _opt(status, "status", device, (1,), _WORD))
+                                       _list(slot, "slot", device, None, _I64), shape[0], _status(status, device))
     if rc:
         _fail(rc)
 
@@ -132,7 +141,8 @@ def attend(q, k_pages, v_pages, table, cached, q_start, out, *, max_fresh, works
     the keys first[r] .. cached[r] + i, of them the last `window` if that is not 0.  out like q; lse [tokens, heads] f32.
     max_fresh: the host's largest number of new tokens per request (chooses the kernel).  workspace: a uint8 tensor of
     attend_workspace() bytes, one for each call that may run at the same time."""
-    _word(max_fresh, window)
+    if not (-_MOST <= max_fresh <= _MOST and -_MOST <= window <= _MOST):
+        _too_wide(max_fresh, window)
     device = _cuda(q)
     store = _store(k_pages, v_pages)
     shape, stride, to = q.shape, q.stride(), out.stride()
@@ -148,7 +158,7 @@ def attend(q, k_pages, v_pages, table, cached, q_start, out, *, max_fresh, works
         device.index, _stream(stream, device), C.byref(store), q.data_ptr(), _DTYPE[q.dtype], stride[0], stride[1], shape[1], _list(table, "table", device),
         table.shape[1], _list(cached, "cached", device, rows), _opt(first, "first", device, rows), _list(q_start, "q_start", device, (rows[0] + 1,)), rows[0], shape[0],
         max_fresh, scale, window, out.data_ptr(), to[0], to[1], _opt(lse, "lse", device, shape[:2], _F32), _list(workspace, "workspace", device, None, torch.uint8),
-        workspace.numel(), _opt(status, "status", device, (1,), _WORD))
+        workspace.numel(), _status(status, device))
     if rc:
         _fail(rc)
 
@@ -168,7 +178,7 @@ def verify_drafts(p, tok, q_start, out, n_out, *, q=None, uniform=None, status=N
     n, vocab = p.shape
     rc = engine.lib().ava_verify_drafts(
         device.index, _stream(stream, device), p.data_ptr(), max(p.stride(0), vocab), None if q is None else q.data_ptr(), vocab if q is None else max(q.stride(0), vocab),
-        _list(tok, "tok", device, (n,), _WORD), _list(q_start, "q_start", device, (rows[0] + 1,)), rows[0], n, vocab, _opt(uniform, "uniform", device, (n,), _F64),
-        out.shape[1], _list(out, "out", device, None, _WORD), _list(n_out, "n_out", device, rows), _opt(status, "status", device, (1,), _WORD))
+        _words(tok, "tok", device, (n,)), _list(q_start, "q_start", device, (rows[0] + 1,)), rows[0], n, vocab, _opt(uniform, "uniform", device, (n,), _F64),
+        out.shape[1], _words(out, "out", device), _list(n_out, "n_out", device, rows), _status(status, device))
     if rc:
         _fail(rc)
