@@ -523,6 +523,19 @@ def test_attend_the_types_largest_values_in_hidden_places_do_not_leak(T, S, dt, 
     assert T.equal(out[keep], clean[0][keep]) and T.equal(lse[keep], clean[1][keep])
 
 
+@pytest.mark.parametrize("dt,max_fresh", [("f32-bf16", 2), ("f32-bf16", 200), ("bf16-bf16", 200), ("f32-f32", 2)])
+def test_attend_more_requests_than_the_line_keeps_sums_for(T, S, dt, max_fresh):
+    """Several requests to a sum (more than 2048 of them), many without new tokens, one long one among them; either kernel."""
+    rng = np.random.default_rng(8)
+    lengths = [(int(rng.integers(0, 40)), int(rng.integers(0, 3)) * int(rng.random() < 0.6)) for _ in range(4500)]
+    lengths[3001] = (5000, 130)
+    lengths[-1] = (0, 1)
+    x = attend_inputs(T, rng, lengths, 2, 1, 64, 16, dt)
+    out, lse = call_attend(T, S, x, 0.125, max_fresh=max_fresh)
+    check_attend(T, x, out, lse, 0.125, only=set(range(0, 4500, 61)) | {3000, 3001, 3002, 4498, 4499})
+    assert T.isfinite(out.float()).all() and not (lse == 7).any()
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("hs,fresh", [(32, 1), (64, 2), (64, 150), (128, 70)])
 @pytest.mark.parametrize("scale", [0.125, -0.3, 0.0])
@@ -617,6 +630,67 @@ def test_attend_on_two_streams_and_in_graphs(T, S, dt, fresh):
 
 
 # ---------------------------------------------------------------------------------------------------------- verify
+def test_calls_from_several_threads_at_once(T, S):
+    import threading
+    cases = [("f32-bf16", 64, [(300, 1)] * 5), ("bf16-bf16", 128, [(90, 70), (5, 200)]), ("f32-bf16", 64, [(50, 150)]), ("f32-f32", 32, [(200, 3)] * 4)]
+    inputs = [attend_inputs(T, np.random.default_rng(i), lengths, 4, 2, hs, 16, dt) for i, (dt, hs, lengths) in enumerate(cases)]
+    want = [call_attend(T, S, x, 0.125) for x in inputs]
+    T.cuda.synchronize()
+    got, errors = [None] * len(cases), []
+
+    def work(i):
+        try:
+            stream = T.cuda.Stream()
+            with T.cuda.stream(stream):
+                for _ in range(20):
+                    got[i] = call_attend(T, S, inputs[i], 0.125)
+                try:
+                    S.attend(inputs[i]["q"], inputs[i]["kp"], inputs[i]["vp"], inputs[i]["table"], inputs[i]["cached"], inputs[i]["start"], got[i][0], max_fresh=1,
+                             workspace=T.zeros(16, dtype=T.uint8, device="cuda:0"), scale=0.125, window=i)
+                    errors.append((i, "not refused"))
+                except engine.EngineError as e:                        # each thread has its own error
+                    if "workspace" not in str(e):
+                        errors.append((i, str(e)))
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append((i, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for g, w in zip(got, want):
+        assert T.equal(g[0], w[0]) and T.equal(g[1], w[1])
+
+
+def test_a_process_whose_first_call_is_captured():
+    import subprocess
+    import sys
+    code = '''
+import torch
+from ava_b200 import serving as S
+d = "cuda:0"
+i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=d)
+q = torch.randn(70, 4, 64, device=d).bfloat16()
+k, v = torch.randn(9, 2, 16, 64, device=d).bfloat16(), torch.randn(9, 2, 16, 64, device=d).bfloat16()
+table, cached, start = torch.arange(9, dtype=torch.int32, device=d)[None].contiguous(), i32(60), i32(0, 70)
+out, room = torch.zeros_like(q), torch.zeros(S.attend_workspace(d, 64), dtype=torch.uint8, device=d)
+call = lambda to: S.attend(q, k, v, table, cached, start, to, max_fresh=70, workspace=room, scale=0.125)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    call(out)
+g.replay()
+torch.cuda.synchronize()
+again = torch.zeros_like(q)
+call(again)
+assert out.abs().sum() > 0 and torch.equal(out, again)
+'''
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def plain_verify(p, q, tok, start, u, max_out):
     """In exact order of the definition, f64."""
     out, counts = np.full((len(start) - 1, max_out), -1, np.int64), []
