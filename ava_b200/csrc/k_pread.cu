@@ -14,11 +14,11 @@
 // f32 queries, f32 stores and the softmax weights of f32 queries are three bf16 limbs each (2^-24 of the value; a store's
 // are made as its elements come out of shared memory), and of two limbed operands' nine products the six down to 2^-18 are
 // taken.  Two limbs (2^-17) were not enough: an error of 2e-6 of the read where f32 sums leave 5e-7.
-// Measured (one B200, 6.57 TB/s copy): one token of 256 sequences of 1024 to 2048 keys, 12 heads of 64, f32 over bf16: 183 us
-// for 1.12 GB, 0.93 of the copy rate; one token over 131072 keys 75 us, 0.82 (9 us pass until the first keys are multiplied,
+// Measured (one B200, 6.57 TB/s copy): one token of 256 sequences of 1024 to 2048 keys, 12 heads of 64, f32 over bf16: 181 us
+// for 1.12 GB, 0.93 of the copy rate; one token over 131072 keys 74 us, 0.83 (9 us pass until the first keys are multiplied,
 // 5 us join the parts); drafted runs of up to 6 tokens of 64 requests over 8192 keys, 32 heads on 8 of 128, bf16: 257 us for
-// 1.52 GB, 0.90.  Three short requests: 14.5 us, of which 4 lie before the first fetch (lengths, the line, the piece), 4 in
-// the steps of one warp after another, 2 around the join.
+// 1.52 GB, 0.90.  Three short requests: 11.2 us, of which 4 lie before the first fetch (lengths, the line, the piece) and 3
+// around the join.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -124,10 +124,12 @@ struct Stage {
     }
 };
 
-// tiles of MR rows, cut into stages; stretches of up to eight stages (128 keys) are not cut
+// tiles of MR rows, cut into stages; stretches of up to two stages (32 keys) are not cut.  (Up to eight: three requests of 64
+// keys 14.6 us instead of 11.2, 200 of 100 keys 26.3 instead of 22.9: with few keys a warp's steps one after another cost more
+// than joining; 256 of 1500 are the same.)
 template <int NQ>
 struct Plan {
-    static constexpr int MR = 8 * NQ, KT = STEP, START = 2, SNAP = 8;
+    static constexpr int MR = 8 * NQ, KT = STEP, START = 2, SNAP = 2;
 };
 
 // How the keys come (box 0: by copies).
