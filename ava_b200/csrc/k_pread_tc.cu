@@ -976,8 +976,8 @@ cudaError_t launch_paged_read_tc(int device, cudaStream_t st, const ReadArgs& a,
     *taken = false;
     PoolShape pool;
     // Few rows per key head stay with the warp kernel, whose tiles of 8 to 32 rows read the store once.  Measured at 32 requests
-    // of 4096 keys, 8 key heads (warp kernel / this one): 24 rows 91 / 115 us and 32 rows 140 / 114 us at 128 channels, 32
-    // rows 86 / 101 us and 48 rows 118 / 101 us at 64; f32 queries 24 rows 101 / 150 us, 48 rows 197 / 154 us.
+    // of up to 4096 keys, 8 key heads (warp kernel / this one): 24 rows 90 / 102 us and 32 rows 144 / 104 us at 128 channels,
+    // 32 rows 83 / 85 us and 48 rows 115 / 84 us at 64; f32 queries 32 rows 134 / 136 us, 48 rows 193 / 136 us.
     const int64_t few = a.s.head_size == 128 ? 24 : 32;
     if (a.s.dtype != AVA_BF16 || (a.s.head_size != 64 && !(a.s.head_size == 128 && a.bf16_q)) || (int64_t)a.max_fresh * a.group <= few || !pool_shape(a.s, &pool))
         return cudaSuccess;
